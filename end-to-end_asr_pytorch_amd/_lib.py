@@ -11,7 +11,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(_HERE, "csrc")
 LIB_PATH = os.environ.get("ASR_AMD_LIB") or os.path.join(CSRC, "libasr_hip.so")     # (ASR_AMD_LIB: another build of the same ABI, for A/B runs)
 SOURCES = ["common.hip", "gemm.hip", "ffn.hip", "ffn2.hip", "vocab.hip", "graph_exec.hip", "collective.hip", "dgrad_rows.hip", "attention.hip", "attention_fwd4.hip", "attention_bwd.hip", "attention_bwd4.hip", "norm_embed.hip", "conv.hip", "ctc.hip", "ce.hip", "cif.hip",
-           "backward.hip", "wgrad.hip", "fused_small.hip", "cif_train.hip", "decode.hip", "decode_blocks.hip", "input.hip"]
+           "backward.hip", "wgrad.hip", "fused_small.hip", "cif_train.hip", "decode.hip", "decode_blocks.hip", "cache4.hip", "input.hip"]
 EXTRA_FLAGS = {"cif.hip": ["-ffp-contract=off"],  # bit-exact CIF: product and sum rounded separately, like the reference
                # ffn2.hip: the phase in front of the generated loop keeps its accumulators in VGPRs (the loop's block owns a0-a63 and the
                # compiler places its own AGPRs behind them: 176 + 64 + 64 would not fit a wave at two per SIMD)
@@ -148,6 +148,11 @@ SIGNATURES = {
     "asr_beam_step": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i],
     "asr_beam_reorder_cache": [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i],
     "asr_beam_advance": [_vp, _vp, _vp, _i, _vp, _i, _vp, _vp],
+    "asr_cache4_put": [_vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i],
+    "asr_cache4_get": [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _i, _vp, _i, _i, _i, _i, _i],
+    "asr_cache4_reorder": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i],
+    "asr_cache4_attention_workspace_bytes": [_i, _i, _i, _i, _i, _i],
+    "asr_cache4_attention": [_vp, _vp, _i, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _i64],
     "asr_add2d": [_vp, _vp, _i64, _vp, _i64, _i, _i],
     "asr_add_transposed": [_vp, _vp, _vp, _i, _i, _i, _i64],
     "asr_relu_mask_mul": [_vp, _vp, _vp, _i, _vp, _i64],
@@ -225,6 +230,7 @@ def lib():
         L.asr_ctc_counter_words.restype = ctypes.c_int64
         L.asr_conv_sub1_bwd_w_workspace_floats.restype = ctypes.c_int64
         L.asr_decode_block_workspace_bytes.restype = ctypes.c_int64
+        L.asr_cache4_attention_workspace_bytes.restype = ctypes.c_int64
         L.asr_last_error.restype = ctypes.c_char_p
         L.asr_version.restype = ctypes.c_int
         _lib = L

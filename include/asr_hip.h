@@ -62,7 +62,7 @@ int asr_dropout_apply(void* stream, const float* x, float* y, int N0, int N1, in
 #define ASR_GEMM_C_IS_ZERO 4u   /* the caller's C is already all zeros: a split-K launch (few output tiles, long K) skips its zeroing kernel */
 
 /* ABI revision: 100 = rounds 1-4; 101 = asr_vocab_proj_lse and asr_ctc_loss_fwd_lse removed (asr_vocab_proj_ctc + asr_ctc_loss_fwd_table
- * replace them), asr_launch_budget_current added; 102 = asr_attn_ffn_fwd added.  A binder checks this before it resolves symbols. */
+ * replace them), asr_launch_budget_current added; 102 = asr_attn_ffn_fwd added; 103 = asr_cache4_* added.  A binder checks this before it resolves symbols. */
 int asr_version(void);
 /* Deterministic mode (also ASR_AMD_DETERMINISTIC=1 in the environment): the forward GEMMs stop splitting K across workgroups (float
  * atomics in arrival order) and the weight gradient's bias side product takes its single-writer form; the weight gradient itself
@@ -638,6 +638,41 @@ int asr_beam_reorder_cache(void* stream, void* cache, const int64_t* parent, con
                            int dtype);
 int asr_beam_advance(void* stream, int32_t* state, int32_t* k_len, int N, const int64_t* cur, int eos, unsigned char* finished,
                      int64_t* len_decoded);
+
+/* ---- K / V cache held in 4 bits ------------------------------------------------------------------------------------------------
+ * A cache of n_kv x N x h rows of Tmax slots (kv = K of layer 0, V of layer 0, K of layer 1, ...; h = key heads): a slot is the 64 values of
+ * one head of one token.
+ *   codes  uint8 [n_kv, N, h, Tmax, 32]   signed 4-bit codes: byte j holds value 2j in its low nibble and value 2j + 1 in its high one
+ *   meta   bf16  [n_kv, N, h, Tmax, 2]    (scale, mid);  the value a code stands for is mid + scale * code
+ * Both contiguous; codes start on 16 bytes, meta on 4.  4.5 bits a value.  Quantising (asr_cache4_put), per slot:
+ *   span = max - min (f32);  scale = bf16(span / 15), 0 where span < 2^-100;  mid = bf16(min + 8 * scale)
+ *   code = (x - mid) / scale rounded to the nearest integer, ties to even - decided exactly, not from a rounded quotient -, cut to [-8, 7]
+ *   (0 where scale is 0: a constant slot reads back as bf16 of its value).  A slot with a NaN or an infinity, or whose span overflows f32,
+ *   gets scale = mid = NaN and reads back as NaN; where it is masked it is never looked at.
+ * asr_cache4_put:  x (f32 | bf16) [n_kv, N, h, L, 64] by element strides s_kv / s_n / s_head / s_tok, the 64 values of a row adjacent, rows on
+ *   16 bytes (strides multiples of 8 in bf16, 4 in f32): token i < n_new[n] goes to slot pos[n * pos_stride] + i.  pos NULL: 0; pos_stride 0:
+ *   one position for all rows (&state[0] of the decoding step), 1: int32 [N].  n_new NULL: all L.  A slot outside [0, Tmax) is not written, and
+ *   slots that no token goes to are left as they were.
+ * asr_cache4_get:  the inverse: out[.., i, :] = the values of slot pos[..] + i for i < n_tok[n], zeros behind (and for slots outside the cache).
+ * asr_cache4_reorder:  the rows of utterance b, b * beam .. b * beam + beam - 1 of the N = B * beam rows, re-gathered by `parent` (int64
+ *   [N], global row ids) for positions <= state[0], like asr_beam_reorder_cache; out_codes / out_meta = codes / meta: in place; another cache:
+ *   its positions > state[0] are left as they were.  beam <= 8.
+ * asr_cache4_attention:  asr_attention_fwd over one K and one V cache of N rows: q (f32 | bf16) [N, h, Lq, 64] by element strides, PRE-MULTIPLIED by
+ *   log2(e)/sqrt(64) as there; h a multiple of h_kv, query head i reads key head i / (h / h_kv); ctx [N, Lq, h * 64] in q's dtype; lse f32
+ *   [N, h, Lq] (base 2) or NULL.  Slot j of row n is visible iff j < k_len[n] (int32 [N], cut to [0, T]; NULL: T) and, with `causal`, j <=
+ *   k_len[n] - Lq + i for query i: the Lq queries are the last tokens of the row.  A query that sees nothing gets zeros and lse = -inf.
+ *   Masked slots may hold anything.  workspace: asr_cache4_attention_workspace_bytes() bytes (0: none needed), contents irrelevant, not shared
+ *   by two launches that may run concurrently. */
+int asr_cache4_put(void* stream, const void* x, int x_dtype, int64_t s_kv, int64_t s_n, int64_t s_head, int64_t s_tok, void* codes, void* meta,
+                   const int32_t* pos, int pos_stride, const int32_t* n_new, int n_kv, int N, int h, int L, int Tmax);
+int asr_cache4_get(void* stream, const void* codes, const void* meta, void* out, int out_dtype, int64_t s_kv, int64_t s_n, int64_t s_head,
+                   int64_t s_tok, const int32_t* pos, int pos_stride, const int32_t* n_tok, int n_kv, int N, int h, int L, int Tmax);
+int asr_cache4_reorder(void* stream, const void* codes, const void* meta, void* out_codes, void* out_meta, const int64_t* parent,
+                       const int32_t* state, int n_kv, int B, int beam, int h, int Tmax);
+int64_t asr_cache4_attention_workspace_bytes(int N, int h, int h_kv, int Lq, int T, int dtype);
+int asr_cache4_attention(void* stream, const void* q, int dtype, int64_t s_n, int64_t s_head, int64_t s_tok, const void* k_codes,
+                         const void* k_meta, const void* v_codes, const void* v_meta, void* ctx, float* lse, int N, int h, int h_kv, int Lq, int T,
+                         const int32_t* k_len, int causal, void* workspace, int64_t workspace_bytes);
 
 /* ---- CIF family, training side (autograd of cif_model.py:44-48, attentionAssigner.py:37-40, conv_encoder.py:33-49) and the tape's
  * gradient bookkeeping; all f32. */
