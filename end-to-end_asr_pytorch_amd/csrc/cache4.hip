@@ -40,7 +40,6 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
     *reinterpret_cast<f32x4*>(p + 4) = f32x4{v[4], v[5], v[6], v[7]};
 }
 
-// lane exchange inside groups of 8 lanes: xor 1, xor 2 (quad_perm), then the mirror image in the half row (the quads hold one value each by then)
 template <int CTRL> __device__ __forceinline__ float dpp_f(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
 }
@@ -49,93 +48,110 @@ template <int CTRL> __device__ __forceinline__ void minmax_step(float& lo, float
     hi = fmaxf(hi, dpp_f<CTRL>(hi));
     bad += dpp_f<CTRL>(bad);
 }
+// d / s with one correction: the quotient rounded to nearest (where it has few bits - on a border k + 1/2 - exactly that), rs = 1 / s to an ulp or two
+__device__ __forceinline__ float quotient(float d, float s, float rs) {
+    const float y = d * rs;
+    return __builtin_fmaf(__builtin_fmaf(-y, s, d), rs, y);
+}
 
-// The codes of 8 values of a row whose 64 values lie in 8 neighbouring lanes: -> the 32-bit word of nibbles, and the row's (scale, mid).
-// Every decision is that of (x - mid) / scale computed exactly.  The quick form (one subtraction, one multiplication by the reciprocal) is
-// off by at most 2^-18 for quotients up to 8; only where it comes within 2^-16 of a border is the exact residual looked at.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& meta) {
+// The codes of 16 values of a row whose 64 values lie in 4 neighbouring lanes: -> the two 32-bit words of nibbles, and the row's (scale, mid).
+// Every decision is that of (x - mid) / scale computed exactly.  The corrected quotient settles it unless the subtraction was rounded and
+// the quotient is next to a border:
+//   bf16  x and mid have 8 bits, so d = x - mid is exact unless one of them is 2^-16 of the other.  |mid| is 0 or at least 2^-6 scale and |x|
+//         at most 17 scale; a tiny x leaves d = -mid, which can only matter if mid itself lies on a border.  Elsewhere a quotient that is
+//         not on a border is 2^-20 away from it or more, and its error below 8 is under 2^-22.
+//   f32   any value may be within the error of a border: those closer than 2^-19 are looked at again.
+// (Exact for all of them, with the rounding error of the subtraction carried along, is 12 instructions a value more: VALU-bound.)
+template <typename T> __device__ __forceinline__ u32x2 quantise16(const float (&x)[16], uint32_t& meta) {
 #pragma clang fp contract(off)
     float lo = x[0], hi = x[0], bad = 0.f;      // bad: 0, or NaN where a value is not finite
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < 16; ++i) {
         lo = fminf(lo, x[i]);
         hi = fmaxf(hi, x[i]);
         bad = __builtin_fmaf(x[i], 0.f, bad);
     }
-    minmax_step<0xB1>(lo, hi, bad);
+    minmax_step<0xB1>(lo, hi, bad);      // quad_perm: lane xor 1, lane xor 2
     minmax_step<0x4E>(lo, hi, bad);
-    minmax_step<0x141>(lo, hi, bad);
     const float span = (hi - lo) + bad;
-    if (!(span < INFINITY)) {
-        meta = 0x7fc07fc0u;
-        return 0u;
-    }
-    const float sc = span < 0x1p-100f ? 0.f : (float)(bf16_t)(span / 15.f);
+    const bool fine = span < INFINITY;
+    const float sc = span < 0x1p-100f || !fine ? 0.f : (float)(bf16_t)(span / 15.f);
     const float mid = (float)(bf16_t)(lo + 8.f * sc);
-    meta = bf16_bits(sc) | (bf16_bits(mid) << 16);
-    if (sc == 0.f) return 0u;
+    meta = fine ? bf16_bits(sc) | (bf16_bits(mid) << 16) : 0x7fc07fc0u;
+    if (sc == 0.f) return u32x2{0u, 0u};
     const float rs = __builtin_amdgcn_rcpf(sc);
-    float k[8], near = 0.f;
+    float k[16], near = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float y = (x[i] - mid) * rs;
+    for (int i = 0; i < 16; ++i) {
+        const float y = quotient(x[i] - mid, sc, rs);
         k[i] = __builtin_rintf(y);
-        near = fmaxf(near, fabsf(y - k[i]));
+        if (sizeof(T) == 4) near = fmaxf(near, fabsf(y - k[i]));
     }
-    if (near > 0.5f - 0x1p-16f) {
+    bool again = near > 0.5f - 0x1p-19f;
+    if (sizeof(T) == 2) {
+        const float ym = quotient(mid, sc, rs);
+        again = __builtin_rintf(2.f * ym) == 2.f * ym && __builtin_rintf(ym) != ym;
+    }
+    if (__builtin_expect(again, 0)) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < 16; ++i) {
             const float d = x[i] - mid, bb = d - x[i], e = (x[i] - (d - bb)) + (-mid - bb);      // d + e = x - mid exactly
-            const float r = __builtin_fmaf(-k[i], sc, d);                                        // exact: k sc has 12 bits
+            const float r = __builtin_fmaf(-k[i], sc, d);                                        // exact next to a border: k sc has 12 bits
             const float g = (fabsf(r) - 0.5f * sc) + (r > 0.f ? e : -e);                         // > 0: the neighbour is nearer
-            if (g > 0.f || (g == 0.f && ((int)k[i] & 1))) k[i] += r > 0.f ? 1.f : -1.f;
+            const bool move = (g > 0.f) | ((g == 0.f) & (((int)k[i] & 1) != 0));
+            k[i] += move ? __builtin_copysignf(1.f, r) : 0.f;
         }
     }
-    uint32_t w = 0;
+    u32x2 w = {0u, 0u};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w |= (uint32_t)(int)(__builtin_amdgcn_fmed3f(k[i], -8.f, 7.f) + 8.f) << (4 * i);
+    for (int i = 0; i < 16; ++i) w[i >> 3] |= (uint32_t)(int)(__builtin_amdgcn_fmed3f(k[i], -8.f, 7.f) + 8.f) << (4 * (i & 7));
     return w ^ 0x88888888u;      // offset code -> two's complement nibble
 }
 
-// Slots of one call: which rows a block works on.  A block is 32 groups of 8 lanes; `tb` (a power of two) tokens of 32 / tb rows side by
-// side, so that a single token per row fills a block as well as a long chunk does; a long chunk's block walks ITER * tb tokens.
+// Slots of one call: which rows a block works on.  A block is 256 / LANES groups of LANES lanes, one row of 64 values each; `tb` (a power of
+// two) tokens of as many rows as fill the block side by side, so that a single token per row fills it as well as a long chunk does; a long
+// chunk's block walks ITER * tb tokens.
 constexpr int ITER = 4;
 struct slots_t {
     const int32_t* pos; const int32_t* n_tok;
-    int pos_stride, N, h, L, Tmax, tb, tb_log2, chunks, rows;
+    int pos_stride, N, h, L, Tmax, tb_log2, rb_log2, chunks, rows;
 };
 struct strides_t { int64_t kv, n, head, tok; };
 
-template <typename F> __device__ __forceinline__ void for_tokens(const slots_t& s, const strides_t& st, F f) {
-    const int chunk = blockIdx.x % s.chunks, group = threadIdx.x >> 3;
-    const int row = (int)(blockIdx.x / s.chunks) * (32 >> s.tb_log2) + (group >> s.tb_log2);
+template <int LANES, typename F> __device__ __forceinline__ void for_tokens(const slots_t& s, const strides_t& st, F f) {
+    const int chunk = s.chunks == 1 ? 0 : blockIdx.x % s.chunks, rows = s.chunks == 1 ? blockIdx.x : blockIdx.x / s.chunks, group = threadIdx.x / LANES;
+    const int row = (rows << s.rb_log2) + (group >> s.tb_log2);
     if (row >= s.rows) return;
     const int head = row % s.h, kn = row / s.h, n = kn % s.N, kv = kn / s.N;
     const int first = s.pos ? s.pos[(int64_t)n * s.pos_stride] : 0;
     const int count = s.n_tok ? clampi(s.n_tok[n], 0, s.L) : s.L;
     const int64_t x0 = kv * st.kv + n * st.n + head * st.head;
     const int64_t c0 = (int64_t)row * s.Tmax;
-    const int t0 = chunk * (s.tb * ITER) + (group & (s.tb - 1));
-#pragma unroll
+    const int tb = 1 << s.tb_log2, t0 = chunk * (tb * ITER) + (group & (tb - 1));
+#pragma unroll 1
     for (int it = 0; it < ITER; ++it) {
-        const int i = t0 + it * s.tb;
-        if (i < s.L) f(i, count, first, x0 + (int64_t)i * st.tok, c0);
+        const int i = t0 + it * tb;
+        if (i >= s.L) break;
+        f(i, count, first, x0 + (int64_t)i * st.tok, c0);
     }
 }
 
 template <typename T>
 __global__ __launch_bounds__(256) void cache4_put_kernel(const T* __restrict__ x, strides_t st, uint32_t* __restrict__ codes,
                                                          uint32_t* __restrict__ meta, slots_t s) {
-    const int l8 = threadIdx.x & 7;
-    for_tokens(s, st, [&](int i, int count, int first, int64_t xo, int64_t c0) {
+    const int l4 = threadIdx.x & 3;
+    for_tokens<4>(s, st, [&](int i, int count, int first, int64_t xo, int64_t c0) {
         const int64_t slot = (int64_t)first + i;
-        if (i >= count || slot < 0 || slot >= s.Tmax) return;      // (one token's 8 lanes agree)
-        float v[8];
-        load8(x + xo + l8 * 8, v);
+        if (i >= count || slot < 0 || slot >= s.Tmax) return;      // (one token's 4 lanes agree)
+        float v[16], a[8], b[8];
+        load8(x + xo + l4 * 16, a);
+        load8(x + xo + l4 * 16 + 8, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = b[j]; }
         uint32_t m;
-        const uint32_t w = quantise8(v, m);
-        codes[(c0 + slot) * 8 + l8] = w;
-        if (l8 == 0) meta[c0 + slot] = m;
+        const u32x2 w = quantise16<T>(v, m);
+        *reinterpret_cast<u32x2*>(codes + (c0 + slot) * 8 + l4 * 2) = w;
+        if (l4 == 0) meta[c0 + slot] = m;
     });
 }
 
@@ -143,7 +159,7 @@ template <typename T>
 __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, strides_t st, const uint32_t* __restrict__ codes,
                                                          const uint32_t* __restrict__ meta, slots_t s) {
     const int l8 = threadIdx.x & 7;
-    for_tokens(s, st, [&](int i, int count, int first, int64_t xo, int64_t c0) {
+    for_tokens<8>(s, st, [&](int i, int count, int first, int64_t xo, int64_t c0) {
         const int64_t slot = (int64_t)first + i;
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
         if (i < count && slot >= 0 && slot < s.Tmax) {
@@ -157,31 +173,39 @@ __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, st
 }
 
 // ---- re-gathering by parent ------------------------------------------------------------------------------------------------------------
-// A group is one (kv, utterance, head); a thread owns one piece of one position (a 16-byte half of its codes, or its meta word) for all
-// `beam` rows: it reads every source row's piece before it writes any, so source and destination may be the same cache.
-template <typename V> __device__ __forceinline__ void regather(const V* src, V* dst, const int (&from)[8], int64_t row_stride, int beam, bool in_place) {
-    V v[8];
+// A group is one (kv, utterance, head).  A block takes 256 pieces of its positions - 16-byte halves of the codes, or meta words - and a thread
+// its piece for all the beam's rows: it reads every source row's before it writes any, so source and destination may be the same cache.  The
+// parents are the same for a whole block: scalar loads, row addresses in scalar registers.
+template <typename V, int BEAM> __device__ __forceinline__ void regather(const V* src, V* dst, const int64_t* parent, int64_t first, int64_t row, int beam, unsigned u,
+                                                                         bool in_place) {
+    V v[BEAM];
+    int from[BEAM];
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-        if (r < beam && !(in_place && from[r] == r)) v[r] = src[(int64_t)from[r] * row_stride];
+    for (int r = 0; r < BEAM; ++r) {
+        from[r] = r < beam ? clampi((int)(parent[r] - first), 0, beam - 1) : r;
+        if (r < beam && !(in_place && from[r] == r)) v[r] = (src + (int64_t)from[r] * row)[u];
+    }
 #pragma unroll
-    for (int r = 0; r < 8; ++r)
-        if (r < beam && !(in_place && from[r] == r)) dst[(int64_t)r * row_stride] = v[r];
+    for (int r = 0; r < BEAM; ++r)
+        if (r < beam && !(in_place && from[r] == r)) (dst + (int64_t)r * row)[u] = v[r];
 }
 
+template <int BEAM>
 __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes, const uint32_t* meta, u32x4* out_codes, uint32_t* out_meta,
                                                              const int64_t* __restrict__ parent, const int32_t* __restrict__ state, int B,
-                                                             int beam, int h, int Tmax, int chunks, bool in_place) {
-    const int n = clampi(state[0] + 1, 0, Tmax);
-    const int u = (int)(blockIdx.x % chunks) * 256 + threadIdx.x;
-    if (u >= 3 * n) return;
-    const int grp = blockIdx.x / chunks, hd = grp % h, kb = grp / h, b = kb % B, kv = kb / B;
-    int from[8];
-#pragma unroll
-    for (int r = 0; r < 8; ++r) from[r] = r < beam ? clampi((int)(parent[(int64_t)b * beam + r] - (int64_t)b * beam), 0, beam - 1) : 0;
-    const int64_t row0 = (((int64_t)kv * B + b) * beam * h + hd) * Tmax;      // slots in front of the group's first row
-    if (u < 2 * n) regather(codes + row0 * 2 + u, out_codes + row0 * 2 + u, from, (int64_t)h * Tmax * 2, beam, in_place);
-    else regather(meta + row0 + (u - 2 * n), out_meta + row0 + (u - 2 * n), from, (int64_t)h * Tmax, beam, in_place);
+                                                             int beam, int h, int Tmax, int chunks_codes, int chunks_meta, int in_place) {
+    const int chunks = chunks_codes + chunks_meta, grp = blockIdx.x / chunks;
+    int chunk = blockIdx.x % chunks;
+    const int hd = grp % h, kb = grp / h, b = kb % B;
+    const int64_t row0 = ((int64_t)kb * beam * h + hd) * Tmax;      // slots in front of the group's first row
+    const int n = clampi(state[0], -1, Tmax - 1) + 1;
+    const bool is_meta = chunk >= chunks_codes;
+    if (is_meta) chunk -= chunks_codes;
+    const unsigned u = chunk * 256u + threadIdx.x;
+    if (u >= (unsigned)(is_meta ? n : 2 * n)) return;
+    parent += (int64_t)b * beam;
+    if (is_meta) regather<uint32_t, BEAM>(meta + row0, out_meta + row0, parent, (int64_t)b * beam, (int64_t)h * Tmax, beam, u, in_place);
+    else regather<u32x4, BEAM>(codes + row0 * 2, out_codes + row0 * 2, parent, (int64_t)b * beam, (int64_t)h * Tmax * 2, beam, u, in_place);
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------------------------
@@ -189,28 +213,26 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
 //     s_j = scale_j (q . c_j) + mid_j sum(q)           p_j = 2^(s_j - m)
 //     o   = (sum_j p_j mid'_j + sum_j (p_j scale'_j) c'_j) / sum_j p_j
 // Both products run over the codes themselves, on the int8 matrix instruction: a nibble masked in place is the byte 16 c, three VALU
-// operations for eight codes, and no value of the cache is ever widened.  The other operand is cut into int8 digits of base 128: the query
+// operations for eight codes, and no value of the cache is ever widened.  The other operand is cut into int8 digits of base 256: the query
 // once per launch (relative to its largest element), the weights w_j = p_j scale'_j once per tile of 64 tokens (relative to the tile's
-// largest, so a tile of small weights keeps its precision).  ND = 2 digits for bf16 queries (a step of 2^-14 of the largest, below the 2^-9
-// that a bf16 weight is rounded by), 3 for f32 (2^-21).  The products are exact int32; softmax statistics and the output are f32.
+// largest, so a tile of small weights keeps its precision).  ND = 2 digits for bf16 queries (half a step is 2^-16 of the largest, below the
+// 2^-9 that a bf16 weight is rounded by), 3 for f32 (2^-24).  The products are exact int32; softmax statistics and the output are f32.
 //
 // A wave owns 64 tokens at a time, token = lane: the query operand of each of a tile's four QK instructions is zero except in the four rows
 // whose results land in the sixteen lanes of the right tokens, so one accumulator collects 64 tokens x (2 queries x 2 digits, or 1 x 3).
-// The weights go through LDS (one byte per lane, query and digit) into the A operand of the PV product, whose rows are (query, digit) and
-// whose B operand - 16 tokens of one channel per lane - is what ds_read_b64_tr_b4 makes of the tile's row-major codes.
+// The weights go through LDS (16 bytes per token: all digits of all queries) into the A operand of the PV product - ds_read_b64_tr_b8 turns
+// them into rows (query, digit) - whose B operand, 16 tokens of one channel per lane, is what ds_read_b64_tr_b4 makes of the tile's
+// row-major codes.
 // The running reference m of a query is renewed only when a score passes it by 2^32 (weights are f32 and scaled per tile: nothing needs
-// them below 1), so a tile costs one reduction across the wave per query, the largest weight's.
+// them below 1), so a tile costs one reduction across the wave per query, the largest weight's, and four queries share its steps.
+// The next tile's loads are issued before the present one is worked on, the first tile's before the query is.
 template <int ND> struct Digits {
-    static constexpr float UNIT = ND == 2 ? 127.f * 128.f : 127.f * 16384.f;      // the integer that the largest element becomes
+    static constexpr float UNIT = ND == 2 ? 127.f * 256.f : 127.f * 65536.f;      // the integer that the largest element becomes
+    static constexpr int BIAS = ND == 2 ? 0x80 : 0x8080;                          // u + BIAS, its lower bytes' sign bits inverted: the digits, lowest first
     static constexpr int QPP = ND == 2 ? 2 : 1;                                   // queries per accumulator
-    // digit `d` (0 = highest) of |u| <= UNIT
-    static __device__ __forceinline__ int get(int u, int d) {
-        if (ND == 2) return d == 0 ? (u + 64) >> 7 : (u << 25) >> 25;
-        const int r = (u << 18) >> 18;
-        return d == 0 ? (u + 8192) >> 14 : d == 1 ? (r + 64) >> 7 : (r << 25) >> 25;
-    }
-    static __device__ __forceinline__ float join(int a, int b, int c) {
-        return ND == 2 ? (float)((a << 7) + b) : __builtin_fmaf((float)a, 16384.f, (float)((b << 7) + c));
+    static __device__ __forceinline__ float join(int d0, int d1, int d2) {
+        const float low = (float)((d1 << 8) + d0);
+        return ND == 2 ? low : __builtin_fmaf((float)d2, 65536.f, low);
     }
 };
 
@@ -219,66 +241,127 @@ struct attn4_t {
     const u32x4* kc; const uint32_t* km; const u32x4* vc; const uint32_t* vm;
     void* ctx; float* lse; float* part;
     const int32_t* k_len;
-    int N, h, h_kv, Lq, T, causal, splits, qtiles, rows, waves;
+    int N, h, h_kv, Lq, T, splits, qtiles, rows, waves;
 };
 constexpr int PART = 66;      // floats of a partial result: 64 outputs (not divided), reference, sum
+constexpr float NO_REF = -3.4028234663852886e38f;
 
 // position of element k of 16 in the byte order that unpacking leaves: low nibbles of the first word, its high ones, then the second word's
 __device__ __forceinline__ int unpack_pos(int k) { return (k & 8) + (k & 1) * 4 + ((k >> 1) & 3); }
 __device__ __forceinline__ i32x4 unpack16(uint32_t w0, uint32_t w1) {
     return i32x4{(int)((w0 << 4) & 0xf0f0f0f0u), (int)(w0 & 0xf0f0f0f0u), (int)((w1 << 4) & 0xf0f0f0f0u), (int)(w1 & 0xf0f0f0f0u)};
 }
-template <int CTRL, int ROWS> __device__ __forceinline__ uint32_t dpp_umax(uint32_t x) {
-    return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
+
+// ---- reductions over the wave: v_permlane32_swap / v_permlane16_swap exchange halves / rows of two registers, the 16 lanes of a row by DPP ----
+struct MaxPos {      // non-negative floats as their bit patterns (a NaN stays the largest)
+    static __device__ __forceinline__ uint32_t f(uint32_t a, uint32_t b) { return max(a, b); }
+};
+struct MaxF {
+    static __device__ __forceinline__ uint32_t f(uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    }
+};
+struct SumF {
+    static __device__ __forceinline__ uint32_t f(uint32_t a, uint32_t b) {
+        return __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b));
+    }
+};
+template <typename OP, int CTRL> __device__ __forceinline__ uint32_t dpp_step(uint32_t x) {
+    return OP::f(x, (uint32_t)__builtin_amdgcn_update_dpp((int)x, (int)x, CTRL, 0xf, 0xf, false));
 }
-// largest of 64 non-negative floats (as their bit patterns), the same for all lanes
-__device__ __forceinline__ float wave_max_pos(float v) {
+template <typename OP> __device__ __forceinline__ uint32_t row16(uint32_t x) {      // row_ror 8, 4, 2, 1
+    x = dpp_step<OP, 0x128>(x);
+    x = dpp_step<OP, 0x124>(x);
+    x = dpp_step<OP, 0x122>(x);
+    return dpp_step<OP, 0x121>(x);
+}
+template <typename OP> __device__ __forceinline__ uint32_t swap32(uint32_t a, uint32_t b) {      // lanes 0..31: a's both halves, 32..63: b's
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    return OP::f(r[0], r[1]);
+}
+template <typename OP> __device__ __forceinline__ uint32_t swap16(uint32_t a, uint32_t b) {      // even rows: a's row pair, odd rows: b's
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    return OP::f(r[0], r[1]);
+}
+template <typename OP> __device__ __forceinline__ float wave_all(float v) {      // the same for all lanes
     uint32_t x = __builtin_bit_cast(uint32_t, v);
-    x = dpp_umax<0x121, 0xf>(x);      // row_ror 1, 2, 4, 8: every lane has its row's
-    x = dpp_umax<0x122, 0xf>(x);
-    x = dpp_umax<0x124, 0xf>(x);
-    x = dpp_umax<0x128, 0xf>(x);
-    x = dpp_umax<0x142, 0xa>(x);      // row_bcast 15 into rows 1 and 3, row_bcast 31 into rows 2 and 3
-    x = dpp_umax<0x143, 0xc>(x);
-    return __builtin_bit_cast(float, __builtin_amdgcn_readlane((int)x, 63));
+    x = swap32<OP>(x, x);
+    x = swap16<OP>(x, x);
+    return __builtin_bit_cast(float, row16<OP>(x));
 }
+// four values at once: row c of the result holds value c's, 9 steps instead of 24
+template <typename OP> __device__ __forceinline__ float wave_four(float v0, float v1, float v2, float v3) {
+    const uint32_t a = swap32<OP>(__builtin_bit_cast(uint32_t, v0), __builtin_bit_cast(uint32_t, v2));
+    const uint32_t b = swap32<OP>(__builtin_bit_cast(uint32_t, v1), __builtin_bit_cast(uint32_t, v3));
+    return __builtin_bit_cast(float, row16<OP>(swap16<OP>(a, b)));
+}
+
 __device__ __forceinline__ void wave_lds_fence() {      // LDS written by other lanes of this wave
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local");
 }
+typedef __attribute__((address_space(3))) i32x2 lds_i32x2;
 
-template <typename T, int ND, int NQ>
+struct tile4_t { u32x4 kw[2], vw[2]; uint32_t km, vm; };
+// a tile's 64 tokens, cut to `last` (what is behind the row's last token is masked where it is used)
+__device__ __forceinline__ void load_tile(tile4_t& t, const u32x4* kc, const u32x4* vc, const uint32_t* km, const uint32_t* vm, int t0, int last, int lane) {
+    const int n16 = lane & 15, c = lane >> 4;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        t.kw[j] = kc[(unsigned)min(t0 + 32 * j + 16 * (c >> 1) + n16, last) * 2u + (c & 1)];
+        t.vw[j] = vc[(unsigned)min(t0 + 32 * j + (lane >> 1), last) * 2u + (lane & 1)];
+    }
+    const unsigned tok = min(t0 + lane, last);
+    t.km = km[tok];
+    t.vm = vm[tok];
+}
+
+template <typename T, int ND, int NQ, bool CAUSAL>
 __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
     using D = Digits<ND>;
     constexpr int PASSES = (NQ + D::QPP - 1) / D::QPP, SLOTS = NQ > 4 ? 2 : 1;
     static_assert(ND == 2 ? NQ <= 8 : NQ <= 4, "16 rows of (query, digit)");
     extern __shared__ __align__(16) unsigned char lds[];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, W = a.waves, n16 = lane & 15, c = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = a.waves, n16 = lane & 15, c = lane >> 4;
     // block -> (row, query tile, split): the query tiles of one stream of keys follow each other at a distance of 8 blocks (one XCD's L2)
-    const int per8 = 8 * a.qtiles, oct = blockIdx.x / per8, rest = blockIdx.x % per8;
-    const int stream = oct * 8 + (rest & 7), qt = rest >> 3;
+    int stream = blockIdx.x, qt = 0;
+    if (a.qtiles > 1) {
+        const int per8 = 8 * a.qtiles, oct = stream / per8, rest = stream - oct * per8;
+        stream = oct * 8 + (rest & 7);
+        qt = rest >> 3;
+    }
     if (stream >= a.rows * a.splits) return;
-    const int row = stream / a.splits, split = stream % a.splits, n = row / a.h_kv, hk = row % a.h_kv;
+    const int row = a.splits == 1 ? stream : stream / a.splits, split = stream - row * a.splits, n = a.h_kv == 1 ? row : row / a.h_kv, hk = row - n * a.h_kv;
+    const int64_t base = (int64_t)row * a.T;
+    const u32x4* kc = a.kc + base * 2;
+    const u32x4* vc = a.vc + base * 2;
+    const uint32_t* km = a.km + base;
+    const uint32_t* vm = a.vm + base;
+    int tile = split * W + wave;
+    tile4_t cur;
+    if (tile * 64 < a.T) load_tile(cur, kc, vc, km, vm, tile * 64, a.T - 1, lane);      // (before the row's length is there: inside the cache either way)
     const int klen = a.k_len ? clampi(a.k_len[n], 0, a.T) : a.T, tiles = (klen + 63) >> 6;
-    if (split > 0 && split >= tiles) return;      // (the joining launch knows which splits have a tile)
+    if (split > 0 && split * W >= tiles) return;      // (the joining launch knows which splits have a tile)
     const int group = a.h / a.h_kv, Q = group * a.Lq, q0 = qt * NQ, nq = min(NQ, Q - q0);
 
     unsigned char* sm_v = lds + wave * 3072;              // 64 rows of 32 bytes, the halves of rows 8 .. 15 of 16 exchanged
-    unsigned char* sm_p = sm_v + 2048;                    // 16 rows (query, digit) of 64 token bytes
+    unsigned char* sm_p = sm_v + 2048;                    // 64 tokens x 16 bytes: the digits of the weights
     unsigned char* sm_q = lds + W * 3072;                 // [NQ][ND][64] digits of the queries
-    float* sm_qs = reinterpret_cast<float*>(sm_q + NQ * ND * 64);      // [NQ][2]: unit of the digits (with the codes' 16), sum
+    float* sm_qs = reinterpret_cast<float*>(sm_q + NQ * ND * 64);      // [NQ][2]: unit of the digits (with the codes' 16), sum in that unit
     for (int j = wave; j < NQ; j += W) {
         float v = 0.f;
         if (j < nq) {
-            const int qi = q0 + j, head = hk * group + qi / a.Lq, i = qi % a.Lq;
-            v = to_f32(static_cast<const T*>(a.q)[n * a.q_n + head * a.q_head + i * a.q_tok + lane]);
+            const int qi = q0 + j, g = a.Lq == 1 ? qi : qi / a.Lq, i = qi - g * a.Lq;
+            v = to_f32(static_cast<const T*>(a.q)[n * a.q_n + (hk * group + g) * a.q_head + i * a.q_tok + lane]);
         }
-        const float top = wave_max(fabsf(v)), sum = wave_sum(v);
-        const int u = top > 0.f ? (int)__builtin_rintf(v * (D::UNIT / top)) : 0;
+        const float top = wave_all<MaxPos>(fabsf(v)), sum = wave_all<SumF>(v);
+        const bool some = !(top < 0x1p-100f);      // (below: a query of zeros)
+        const uint32_t u = some ? (uint32_t)((int)__builtin_rintf(v * (D::UNIT / top)) + D::BIAS) ^ D::BIAS : 0u;
 #pragma unroll
-        for (int d = 0; d < ND; ++d) sm_q[(j * ND + d) * 64 + (lane & 48) + unpack_pos(n16)] = (unsigned char)D::get(u, d);
-        if (lane == 0) { sm_qs[2 * j] = top * (1.f / (16.f * D::UNIT)); sm_qs[2 * j + 1] = sum; }
+        for (int d = 0; d < ND; ++d) sm_q[(j * ND + d) * 64 + (lane & 48) + unpack_pos(n16)] = (unsigned char)(u >> (8 * d));
+        const float unit = some ? top * (1.f / (16.f * D::UNIT)) : 1.f;
+        if (lane == 0) { sm_qs[2 * j] = unit; sm_qs[2 * j + 1] = some ? sum / unit : 0.f; }
     }
     __syncthreads();
     i32x4 qa[PASSES][2][2];      // [j]: tokens 32 j .. 32 j + 31 of the tile, [half]: the first or second 16 of a lane's 32 channels
@@ -299,42 +382,31 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
         unit[q] = sm_qs[2 * q]; qsum[q] = sm_qs[2 * q + 1];
-        m[q] = -3.4028234663852886e38f; l[q] = 0.f; mv[q] = 0.f;
-        lim[q] = a.causal ? klen - (a.Lq - 1) + (q0 + q) % a.Lq : klen;
+        m[q] = NO_REF; l[q] = 0.f; mv[q] = 0.f;
+        lim[q] = CAUSAL ? klen - (a.Lq - 1) + (q0 + q) % a.Lq : klen;
     }
 #pragma unroll
     for (int d = 0; d < 4; ++d)
 #pragma unroll
         for (int s = 0; s < SLOTS; ++s) acc[d][s] = 0.f;
 
-    const int64_t base = (int64_t)row * a.T;
-    const u32x4* kc = a.kc + base * 2;
-    const u32x4* vc = a.vc + base * 2;
-    const uint32_t* km = a.km + base;
-    const uint32_t* vm = a.vm + base;
-    for (int tile = split + wave * a.splits; tile < tiles; tile += a.splits * W) {
-        const int t0 = tile * 64, last = klen - 1;
-        u32x4 kw[2], vw[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {      // (tokens behind the last are read as the last one: their scores are masked below)
-            kw[j] = kc[(unsigned)min(t0 + 32 * j + 16 * (c >> 1) + n16, last) * 2u + (c & 1)];
-            vw[j] = vc[(unsigned)min(t0 + 32 * j + (lane >> 1), last) * 2u + (lane & 1)];
-        }
-        const int tok = t0 + lane;
-        const uint32_t kmeta = km[min(tok, last)];
-        uint32_t vmeta = vm[min(tok, last)];
-        if (tok >= klen) vmeta = 0u;
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int r = 32 * j + (lane >> 1);
-            *reinterpret_cast<u32x4*>(sm_v + r * 32 + (((lane & 1) ^ ((r >> 3) & 1)) << 4)) = vw[j];
-        }
-        // scores
+    const int step = a.splits * W;
+    for (; tile < tiles; tile += step) {
+        const int tok = tile * 64 + lane;
         i32x4 ku[2][2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) { ku[j][0] = unpack16(kw[j][0], kw[j][1]); ku[j][1] = unpack16(kw[j][2], kw[j][3]); }
+        for (int j = 0; j < 2; ++j) {
+            ku[j][0] = unpack16(cur.kw[j][0], cur.kw[j][1]);
+            ku[j][1] = unpack16(cur.kw[j][2], cur.kw[j][3]);
+            const int r = 32 * j + (lane >> 1);
+            *reinterpret_cast<u32x4*>(sm_v + r * 32 + (((lane & 1) ^ ((r >> 3) & 1)) << 4)) = cur.vw[j];
+        }
+        const bool live = tok < klen;      // (what is behind the last token may be anything)
+        const uint32_t kmeta = live ? cur.km : 0u, vmeta = live ? cur.vm : 0u;
+        const float hide = live ? 0.f : -INFINITY;
+        if (tile + step < tiles) load_tile(cur, kc, vc, km, vm, (tile + step) * 64, klen - 1, lane);
         const float ksc = meta_scale(kmeta), kmid = meta_mid(kmeta), vsc = meta_scale(vmeta), vmid = meta_mid(vmeta);
-        float s[NQ];
+        float s[NQ], e[NQ], top = -INFINITY;
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
             i32x4 dot = {0, 0, 0, 0};
@@ -342,27 +414,25 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
             for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[p][j][half], ku[j][half], dot, 0, 0, 0);
-            if (D::QPP == 2) {
-                s[2 * p] = D::join(dot[0], dot[1], 0);
-                if (2 * p + 1 < NQ) s[2 * p + 1] = D::join(dot[2], dot[3], 0);
-            } else {
-                s[p] = D::join(dot[0], dot[1], dot[2]);
-            }
+#pragma unroll
+            for (int i = 0; i < D::QPP; ++i)
+                if (D::QPP * p + i < NQ) s[D::QPP * p + i] = D::QPP == 2 ? D::join(dot[2 * i], dot[2 * i + 1], 0) : D::join(dot[0], dot[1], dot[2]);
         }
-        bool up = false;
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-            s[q] = __builtin_fmaf(s[q] * unit[q], ksc, kmid * qsum[q]);
-            s[q] = tok < lim[q] ? s[q] : -INFINITY;
-            up = up || s[q] > m[q] + 32.f;
+            s[q] = __builtin_fmaf(s[q], ksc, __builtin_fmaf(kmid, qsum[q], hide));      // in units of unit[q]
+            if (CAUSAL) s[q] = tok < lim[q] ? s[q] : -INFINITY;
+            e[q] = __builtin_fmaf(s[q], unit[q], -m[q]);
+            top = fmaxf(top, e[q]);
         }
-        if (__builtin_amdgcn_ballot_w64(up)) {
+        if (__builtin_amdgcn_ballot_w64(top > 32.f)) {
             float al[NQ];
 #pragma unroll
             for (int q = 0; q < NQ; ++q) {
-                const float mn = fmaxf(m[q], wave_max(s[q]));
+                const float mn = fmaxf(m[q], wave_all<MaxF>(s[q]) * unit[q]);
                 al[q] = __builtin_amdgcn_exp2f(m[q] - mn);
                 m[q] = mn; l[q] *= al[q]; mv[q] *= al[q];
+                e[q] = __builtin_fmaf(s[q], unit[q], -mn);
             }
 #pragma unroll
             for (int sl = 0; sl < SLOTS; ++sl) {
@@ -375,34 +445,54 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
             }
         }
         // weights -> digits
-        float wunit[SLOTS];
+        float w[4 * SLOTS], wunit[SLOTS], inv[SLOTS];
+        uint32_t u[4 * SLOTS];
 #pragma unroll
-        for (int sl = 0; sl < SLOTS; ++sl) wunit[sl] = 0.f;
+        for (int q = 0; q < 4 * SLOTS; ++q) {
+            w[q] = 0.f;
+            if (q < NQ) {
+                const float p = __builtin_amdgcn_exp2f(e[q < NQ ? q : 0]);
+                const bool seen = !CAUSAL || tok < lim[q < NQ ? q : 0];      // (0 * NaN of a token that another query sees must not enter the sums)
+                l[q < NQ ? q : 0] += p;
+                mv[q < NQ ? q : 0] = __builtin_fmaf(p, seen ? vmid : 0.f, mv[q < NQ ? q : 0]);
+                w[q] = p * (seen ? vsc : 0.f);
+            }
+        }
+#pragma unroll
+        for (int sl = 0; sl < SLOTS; ++sl) {
+            const float most = NQ == 1 ? wave_all<MaxPos>(w[0]) : wave_four<MaxPos>(w[4 * sl], w[4 * sl + 1], w[4 * sl + 2], w[4 * sl + 3]);      // of query 4 sl + c
+            inv[sl] = most > 1e-30f ? D::UNIT * __builtin_amdgcn_rcpf(most) : 0.f;
+            wunit[sl] = most * (1.f / (16.f * D::UNIT));
+        }
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-            const float p = __builtin_amdgcn_exp2f(s[q] - m[q]);
-            const bool seen = tok < lim[q];      // (a masked token may hold anything: 0 * NaN must not enter the sums)
-            l[q] += p;
-            mv[q] = __builtin_fmaf(p, seen ? vmid : 0.f, mv[q]);
-            const float w = p * (seen ? vsc : 0.f);
-            const float top = wave_max_pos(w);
-            const float inv = top > 1e-30f ? D::UNIT * __builtin_amdgcn_rcpf(top) : 0.f;
-            const int u = __builtin_bit_cast(int, __builtin_fmaf(w, inv, 12582912.f));      // round to nearest: the integer in the low 22 bits
-            const int prow = 4 * (q & 3) + (ND == 2 ? 2 * (q >> 2) : 0);
-#pragma unroll
-            for (int d = 0; d < ND; ++d) sm_p[(prow + d) * 64 + (lane & 48) + unpack_pos(n16)] = (unsigned char)D::get(u, d);
-            if (c == (q & 3)) wunit[q >> 2] = top * (1.f / (16.f * D::UNIT));
+            const float iq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv[q >> 2]), 16 * (q & 3)));
+            if (ND == 2) u[q] = __builtin_bit_cast(uint32_t, __builtin_fmaf(w[q], iq, 12582912.f + D::BIAS));      // round to nearest: the integer in the low bits
+            else u[q] = (uint32_t)__builtin_fmaf(w[q], iq, D::BIAS + 0.5f) ^ D::BIAS;
         }
-        wave_lds_fence();
-        const i32x4 pa = *reinterpret_cast<const i32x4*>(sm_p + n16 * 64 + c * 16);
+        uint32_t pw[4];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) {
-            const int r = lane;      // group c of 16 lanes: rows 16 c .. 16 c + 15, 8 bytes (16 channels) each, transposed on the way
-            const i32x2 w = __builtin_amdgcn_ds_read_tr4_b64_v2i32((__attribute__((address_space(3))) i32x2*)(
-                (__attribute__((address_space(3))) unsigned char*)sm_v + r * 32 + (((d >> 1) ^ ((r >> 3) & 1)) << 4) + (d & 1) * 8));
-            const i32x4 o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa, unpack16((uint32_t)w[0], (uint32_t)w[1]), i32x4{0, 0, 0, 0}, 0, 0, 0);
+        for (int q = 0; q < 4; ++q) {
+            pw[q] = 0u;
+            if (q < NQ) pw[q] = u[q < NQ ? q : 0];
+            if (ND == 2 && q + 4 < NQ) pw[q] = __builtin_amdgcn_perm(u[q + 4 < NQ ? q + 4 : 0], pw[q], 0x05040100u);
+            if (ND == 2) pw[q] ^= 0x00800080u;
+        }
+        unsigned char* to = sm_p + ((lane & 48) + unpack_pos(n16)) * 16;
+        if (NQ == 1) *reinterpret_cast<uint32_t*>(to) = pw[0];
+        else if (NQ == 2) *reinterpret_cast<u32x2*>(to) = u32x2{pw[0], pw[1]};
+        else *reinterpret_cast<u32x4*>(to) = u32x4{pw[0], pw[1], pw[2], pw[3]};
+        wave_lds_fence();
+        lds_i32x2* from = (lds_i32x2*)((__attribute__((address_space(3))) unsigned char*)sm_p + c * 256 + n16 * 8);
+        const i32x2 p0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(from), p1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(from + 16);
+        const i32x4 pa = {p0[0], p0[1], p1[0], p1[1]};
+#pragma unroll
+        for (int d = 0; d < 4; ++d) {      // 16 channels: group c of 16 lanes reads rows 16 c .. 16 c + 15, 8 bytes each, transposed on the way
+            const i32x2 vt = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)((__attribute__((address_space(3))) unsigned char*)sm_v + lane * 32 +
+                                                                                  (((d >> 1) ^ ((lane >> 3) & 1)) << 4) + (d & 1) * 8));
+            const i32x4 o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa, unpack16((uint32_t)vt[0], (uint32_t)vt[1]), i32x4{0, 0, 0, 0}, 0, 0, 0);
             acc[d][0] = __builtin_fmaf(D::join(o[0], o[1], o[2]), wunit[0], acc[d][0]);
-            if (SLOTS == 2) acc[d][1] = __builtin_fmaf(D::join(o[2], o[3], 0), wunit[SLOTS - 1], acc[d][SLOTS - 1]);
+            if (SLOTS == 2) acc[d][SLOTS - 1] = __builtin_fmaf(D::join(o[2], o[3], 0), wunit[SLOTS - 1], acc[d][SLOTS - 1]);
         }
         wave_lds_fence();
     }
@@ -413,7 +503,7 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
     float* sm_m = sm_o + W * NQ * 64;                 // [W][NQ][2]
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
-        const float lw = wave_sum(l[q]), mw = wave_sum(mv[q]);
+        const float lw = wave_all<SumF>(l[q]), mw = wave_all<SumF>(mv[q]);
         if (lane == 0) { sm_m[(wave * NQ + q) * 2] = m[q]; sm_m[(wave * NQ + q) * 2 + 1] = lw; }
         if (c == (q & 3))
 #pragma unroll
@@ -428,7 +518,7 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
             L = __builtin_fmaf(sm_m[(w * NQ + q) * 2 + 1], f, L);
             o = __builtin_fmaf(sm_o[(w * NQ + q) * 64 + lane], f, o);
         }
-        const int qi = q0 + q, head = hk * group + qi / a.Lq, i = qi % a.Lq;
+        const int qi = q0 + q, g = a.Lq == 1 ? qi : qi / a.Lq, i = qi - g * a.Lq, head = hk * group + g;
         if (a.splits == 1) {
             static_cast<T*>(a.ctx)[(((int64_t)n * a.Lq + i) * a.h + head) * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : o / L);
             if (a.lse && lane == 0) a.lse[((int64_t)n * a.h + head) * a.Lq + i] = L == 0.f ? -INFINITY : M + __log2f(L);
@@ -446,9 +536,9 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(attn4_t a) {
     __shared__ float sm[4][PART];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = a.h / a.h_kv, Q = group * a.Lq;
     const int row = blockIdx.x / Q, qi = blockIdx.x % Q, n = row / a.h_kv, hk = row % a.h_kv;
-    const int klen = a.k_len ? clampi(a.k_len[n], 0, a.T) : a.T, live = max(1, min(a.splits, (klen + 63) >> 6));
+    const int klen = a.k_len ? clampi(a.k_len[n], 0, a.T) : a.T, live = clampi(((klen + 63) / 64 + a.waves - 1) / a.waves, 1, a.splits);
     const float* part = a.part + ((int64_t)row * Q + qi) * a.splits * PART;
-    float M = -3.4028234663852886e38f, L = 0.f, o = 0.f;
+    float M = NO_REF, L = 0.f, o = 0.f;
     for (int s = wave; s < live; s += 4) {
         const float* p = part + (int64_t)s * PART;
         const float v = p[lane], ms = p[64], ls = p[65], mn = fmaxf(M, ms);
@@ -492,14 +582,17 @@ plan_t attn_plan(int rows, int Q, int T, int dtype) {
     return p;
 }
 
-template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, const plan_t& p) {
+template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, const plan_t& p, bool causal) {
     const size_t work = (size_t)p.waves * 3072 + p.nq * (ND * 64 + 8), join = (size_t)p.waves * p.nq * 66 * 4;
     const size_t lds = work > join ? work : join;
-    const int64_t octs = ((int64_t)a.rows * a.splits + 7) / 8;
-    const dim3 grid((unsigned)(octs * 8 * a.qtiles)), block(p.waves * 64);
+    const int64_t streams = (int64_t)a.rows * a.splits;
+    const dim3 grid((unsigned)(a.qtiles == 1 ? streams : (streams + 7) / 8 * 8 * a.qtiles)), block(p.waves * 64);
 #define ASR_C4(NQ)                                                                                      \
     case NQ:                                                                                            \
-        if constexpr (ND == 2 || NQ <= 4) hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ>), grid, block, lds, s, a); \
+        if constexpr (ND == 2 || NQ <= 4) {                                                             \
+            if (causal) hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, true>), grid, block, lds, s, a); \
+            else hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, false>), grid, block, lds, s, a);    \
+        }                                                                                               \
         break;
     switch (p.nq) { ASR_C4(1) ASR_C4(2) ASR_C4(3) ASR_C4(4) ASR_C4(5) ASR_C4(6) ASR_C4(7) ASR_C4(8) }
 #undef ASR_C4
@@ -511,18 +604,19 @@ template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, c
     return 0;
 }
 
-int slots_plan(const char* name, slots_t& s, int64_t& blocks, int n_kv, int N, int h, int L, int Tmax, const int32_t* pos, int pos_stride,
+int slots_plan(const char* name, int lanes, slots_t& s, int64_t& blocks, int n_kv, int N, int h, int L, int Tmax, const int32_t* pos, int pos_stride,
                const int32_t* n_tok) {
     ASR_REQUIRE(n_kv > 0 && N > 0 && h > 0 && L > 0 && Tmax > 0, ASR_ERR_ARG, "%s: bad sizes (n_kv=%d N=%d h=%d L=%d Tmax=%d)", name, n_kv, N, h, L, Tmax);
     ASR_REQUIRE(Tmax <= CACHE4_MAX_T && L <= CACHE4_MAX_T, ASR_ERR_UNSUPPORTED, "%s: more than 2^24 slots", name);
     ASR_REQUIRE(pos_stride == 0 || pos_stride == 1, ASR_ERR_ARG, "%s: pos_stride is 0 (one position for all rows) or 1", name);
     const int64_t rows = (int64_t)n_kv * N * h;
-    int tb = 1, lg = 0;
-    while (tb < 32 && tb < L) { tb *= 2; ++lg; }
-    const int chunks = (L + tb * ITER - 1) / (tb * ITER);
-    blocks = (rows + (32 >> lg) - 1) / (32 >> lg) * chunks;
-    ASR_REQUIRE(rows <= INT32_MAX && blocks <= INT32_MAX, ASR_ERR_UNSUPPORTED, "%s: too many rows", name);
-    s = slots_t{pos, n_tok, pos_stride, N, h, L, Tmax, tb, lg, chunks, (int)rows};
+    const int groups_log2 = lanes == 4 ? 6 : 5;      // rows of 64 values side by side in a block of 256 threads
+    int lg = 0;
+    while (lg < groups_log2 && (1 << lg) < L) ++lg;
+    const int rb_log2 = groups_log2 - lg, chunks = (int)((L + ((int64_t)ITER << lg) - 1) / ((int64_t)ITER << lg));
+    blocks = (rows + (1 << rb_log2) - 1) / (1 << rb_log2) * chunks;
+    ASR_REQUIRE(rows <= INT32_MAX - 64 && blocks <= INT32_MAX, ASR_ERR_UNSUPPORTED, "%s: too many rows", name);
+    s = slots_t{pos, n_tok, pos_stride, N, h, L, Tmax, lg, rb_log2, chunks, (int)rows};
     return 0;
 }
 bool strides_ok(const strides_t& st, int per16) { return st.kv % per16 == 0 && st.n % per16 == 0 && st.head % per16 == 0 && st.tok % per16 == 0; }
@@ -534,7 +628,7 @@ extern "C" int asr_cache4_put(void* stream, const void* x, int x_dtype, int64_t 
     ASR_REQUIRE(x && codes && meta, ASR_ERR_ARG, "cache4_put: null pointer");
     ASR_REQUIRE(x_dtype == ASR_F32 || x_dtype == ASR_BF16, ASR_ERR_ARG, "cache4_put: dtype %d (ASR_F32 or ASR_BF16)", x_dtype);
     slots_t s; int64_t blocks;
-    if (const int rc = slots_plan("cache4_put", s, blocks, n_kv, N, h, L, Tmax, pos, pos_stride, n_new)) return rc;
+    if (const int rc = slots_plan("cache4_put", 4, s, blocks, n_kv, N, h, L, Tmax, pos, pos_stride, n_new)) return rc;
     const strides_t st{s_kv, s_n, s_head, s_tok};
     ASR_REQUIRE(asr_aligned(x, 16) && asr_aligned(codes, 16) && asr_aligned(meta, 4) && strides_ok(st, x_dtype == ASR_F32 ? 4 : 8), ASR_ERR_ALIGN,
                 "cache4_put: rows of x start on 16 bytes, codes on 16, meta on 4");
@@ -554,7 +648,7 @@ extern "C" int asr_cache4_get(void* stream, const void* codes, const void* meta,
     ASR_REQUIRE(out && codes && meta, ASR_ERR_ARG, "cache4_get: null pointer");
     ASR_REQUIRE(out_dtype == ASR_F32 || out_dtype == ASR_BF16, ASR_ERR_ARG, "cache4_get: dtype %d (ASR_F32 or ASR_BF16)", out_dtype);
     slots_t s; int64_t blocks;
-    if (const int rc = slots_plan("cache4_get", s, blocks, n_kv, N, h, L, Tmax, pos, pos_stride, n_tok)) return rc;
+    if (const int rc = slots_plan("cache4_get", 8, s, blocks, n_kv, N, h, L, Tmax, pos, pos_stride, n_tok)) return rc;
     const strides_t st{s_kv, s_n, s_head, s_tok};
     ASR_REQUIRE(asr_aligned(out, 16) && asr_aligned(codes, 16) && asr_aligned(meta, 4) && strides_ok(st, out_dtype == ASR_F32 ? 4 : 8), ASR_ERR_ALIGN,
                 "cache4_get: rows of out start on 16 bytes, codes on 16, meta on 4");
@@ -576,12 +670,17 @@ extern "C" int asr_cache4_reorder(void* stream, const void* codes, const void* m
     ASR_REQUIRE(Tmax <= CACHE4_MAX_T, ASR_ERR_UNSUPPORTED, "cache4_reorder: more than 2^24 slots");
     ASR_REQUIRE((codes == out_codes) == (meta == out_meta), ASR_ERR_ARG, "cache4_reorder: in place means codes and meta both");
     ASR_REQUIRE(asr_aligned(codes, 16) && asr_aligned(out_codes, 16) && asr_aligned(meta, 4) && asr_aligned(out_meta, 4), ASR_ERR_ALIGN, "cache4_reorder: alignment");
-    const int chunks = (int)((3 * (int64_t)Tmax + 255) / 256);
-    const int64_t blocks = (int64_t)n_kv * B * h * chunks;
+    const int chunks_codes = (2 * Tmax + 255) / 256, chunks_meta = (Tmax + 255) / 256;
+    const int64_t blocks = (int64_t)n_kv * B * h * (chunks_codes + chunks_meta);
     ASR_REQUIRE(blocks <= INT32_MAX, ASR_ERR_UNSUPPORTED, "cache4_reorder: too many rows");
-    hipLaunchKernelGGL(cache4_reorder_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<hipStream_t>(stream), static_cast<const u32x4*>(codes),
-                       static_cast<const uint32_t*>(meta), static_cast<u32x4*>(out_codes), static_cast<uint32_t*>(out_meta), parent, state, B, beam, h, Tmax,
-                       chunks, codes == out_codes);
+    hipStream_t hs = static_cast<hipStream_t>(stream);
+#define ASR_C4(BEAM)                                                                                                                                     \
+    hipLaunchKernelGGL((cache4_reorder_kernel<BEAM>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const u32x4*>(codes), static_cast<const uint32_t*>(meta), \
+                       static_cast<u32x4*>(out_codes), static_cast<uint32_t*>(out_meta), parent, state, B, beam, h, Tmax, chunks_codes, chunks_meta, codes == out_codes)
+    if (beam <= 2) ASR_C4(2);
+    else if (beam <= 4) ASR_C4(4);
+    else ASR_C4(8);
+#undef ASR_C4
     ASR_LAUNCH_CHECK("cache4_reorder");
     return 0;
 }
@@ -607,8 +706,8 @@ extern "C" int asr_cache4_attention(void* stream, const void* q, int dtype, int6
     ASR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asr_aligned(workspace, 4)), ASR_ERR_ARG, "cache4_attention: workspace of %lld bytes needed, %lld given",
                 (long long)need, (long long)(workspace ? workspace_bytes : 0));
     attn4_t a{q, s_n, s_head, s_tok, static_cast<const u32x4*>(k_codes), static_cast<const uint32_t*>(k_meta), static_cast<const u32x4*>(v_codes),
-              static_cast<const uint32_t*>(v_meta), ctx, lse, static_cast<float*>(workspace), k_len, N, h, h_kv, Lq, T, causal ? 1 : 0, p.splits, p.qtiles,
+              static_cast<const uint32_t*>(v_meta), ctx, lse, static_cast<float*>(workspace), k_len, N, h, h_kv, Lq, T, p.splits, p.qtiles,
               N * h_kv, p.waves};
     hipStream_t s = static_cast<hipStream_t>(stream);
-    return dtype == ASR_BF16 ? attn_launch<bf16_t, 2>(s, a, p) : attn_launch<float, 3>(s, a, p);
+    return dtype == ASR_BF16 ? attn_launch<bf16_t, 2>(s, a, p, causal != 0) : attn_launch<float, 3>(s, a, p, causal != 0);
 }

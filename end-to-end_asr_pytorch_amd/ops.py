@@ -6,6 +6,7 @@ no arithmetic on the product path is done by torch ops.  There is no CPU fallbac
 """
 import atexit
 import ctypes
+import functools
 import weakref
 import os
 import threading
@@ -1379,21 +1380,27 @@ def beam_advance(state, k_len, cur=None, eos_id=0, finished=None, len_decoded=No
 
 
 # ---- K / V cache held in 4 bits (csrc/cache4.hip) -------------------------------------------------------------------------------
+# (A token's calls are a few microseconds of GPU work each and a step makes dozens of them: these wrappers pass plain integers to ctypes and
+# ask a tensor for each property once - 6-7 us a call on the host instead of 13.)
 class Cache4:
     """A K / V cache in 4 bits (asr_hip.h: asr_cache4_put): `codes` uint8 [n_kv, N, h, Tmax, 32] and `meta` bf16 [n_kv, N, h, Tmax, 2] - or both
-    without the first dimension, one cache (`cache[i]` of a stack: views of the same memory).  4.5 bits a value against 16 or 32."""
-    __slots__ = ("codes", "meta")
+    without the first dimension, one cache (`cache[i]` of a stack: views of the same memory).  4.5 bits a value against 16 or 32.
+    `shape` = (n_kv, N, h, Tmax), n_kv = 1 for one cache."""
+    __slots__ = ("codes", "meta", "shape", "stack", "device")
 
     def __init__(self, codes, meta):
-        if codes.dtype != torch.uint8 or meta.dtype != torch.bfloat16:
+        if codes.dtype is not torch.uint8 or meta.dtype is not torch.bfloat16:
             raise TypeError("Cache4: codes are uint8 and meta bfloat16, got %s and %s" % (codes.dtype, meta.dtype))
-        if codes.dim() not in (4, 5) or codes.shape[-1] != 32 or meta.shape[-1] != 2 or codes.shape[:-1] != meta.shape[:-1]:
-            raise ValueError("Cache4: codes [.., N, h, Tmax, 32] and meta [.., N, h, Tmax, 2], got %s and %s" % (tuple(codes.shape), tuple(meta.shape)))
+        cs, ms = tuple(codes.shape), tuple(meta.shape)
+        if len(cs) not in (4, 5) or cs[-1] != 32 or ms[-1] != 2 or cs[:-1] != ms[:-1]:
+            raise ValueError("Cache4: codes [.., N, h, Tmax, 32] and meta [.., N, h, Tmax, 2], got %s and %s" % (cs, ms))
         if not (codes.is_contiguous() and meta.is_contiguous()):
             raise ValueError("Cache4: codes and meta are contiguous")
-        if codes.device != meta.device:
+        self.device = codes.get_device()
+        if self.device != meta.get_device():
             raise ValueError("Cache4: codes on %s, meta on %s" % (codes.device, meta.device))
-        self.codes, self.meta = codes, meta
+        self.codes, self.meta, self.stack = codes, meta, len(cs) == 5
+        self.shape = cs[:-1] if len(cs) == 5 else (1,) + cs[:-1]
 
     @classmethod
     def empty(cls, n_kv, N, h, Tmax, device):
@@ -1402,72 +1409,70 @@ class Cache4:
         return cls(torch.zeros(lead + (32,), dtype=torch.uint8, device=device), torch.zeros(lead + (2,), dtype=torch.bfloat16, device=device))
 
     def __getitem__(self, i):
-        if self.codes.dim() != 5:
+        if not self.stack:
             raise IndexError("Cache4: one cache, not a stack")
         return Cache4(self.codes[i], self.meta[i])
 
     def __len__(self):
-        return self.codes.shape[0] if self.codes.dim() == 5 else 1
-
-    @property
-    def shape(self):
-        """(n_kv, N, h, Tmax)"""
-        lead = tuple(self.codes.shape[:-1])
-        return lead if len(lead) == 4 else (1,) + lead
+        return self.shape[0]
 
 
-class _on:
-    """the launches inside go to the current stream of the tensors' own device, whichever device is current outside"""
-    __slots__ = ("dev", "guard")
-
-    def __init__(self, what, *ts):
-        _req_cuda(*ts)
-        self.dev = ts[0].device
-        for t in ts:
-            if t is not None and t.device != self.dev:
-                raise ValueError("%s: tensors on %s and %s" % (what, self.dev, t.device))
-
-    def __enter__(self):
-        self.guard = None
-        if self.dev.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.dev)
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _cache4_call(what, fn, cache, ts, args):
+    """fn(stream, *args) on the current stream of the tensors' own device, whichever device is current outside"""
+    dev = cache.device
+    for t in ts:
+        if t is not None and t.get_device() != dev:
+            raise RuntimeError("asr_amd: %s: tensors on %s and %s" % (what, cache.codes.device, t.device))
+    if dev < 0:
+        _req_cuda(cache.codes)
+    if dev != torch._C._cuda_getDevice():
+        with torch.cuda.device(dev):
+            return check(fn(_stream(), *args), what)
+    rc = fn(_stream(), *args)
+    if rc:
+        check(rc, what)
 
 
-def _cache4_slots(what, cache, pos, n_tok):
-    """-> (pos stride); int32 positions (one, or one per row) and counts (one per row)"""
-    N = cache.shape[1]
-    for name, t, ok in (("pos", pos, (1, N)), ("n_new / n_tok", n_tok, (N,))):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous() or t.numel() not in ok):
-            raise ValueError("%s: %s is a contiguous int32 tensor of %s elements" % (what, name, " or ".join(str(v) for v in ok)))
-    return 1 if pos is not None and pos.numel() == N and N > 1 else 0
+def _ptr(t):
+    return None if t is None else t.data_ptr()
 
 
-def _cache4_strides(what, t, sizes):
-    """element strides of [.., L, 64] rows; a dimension of one element has none"""
-    if t.stride(-1) != 1:
+def _cache4_slots(what, N, pos, n_tok):
+    """-> the stride of the positions; int32 positions (one, or one per row) and counts (one per row)"""
+    if n_tok is not None and (n_tok.dtype is not torch.int32 or n_tok.numel() != N or not n_tok.is_contiguous()):
+        raise ValueError("%s: n_new / n_tok is a contiguous int32 tensor of %d elements" % (what, N))
+    if pos is None:
+        return 0
+    n = pos.numel()
+    if pos.dtype is not torch.int32 or (n != N and n != 1) or not pos.is_contiguous():
+        raise ValueError("%s: pos is a contiguous int32 tensor of 1 or %d elements" % (what, N))
+    return 1 if n > 1 else 0
+
+
+def _cache4_strides(what, t):
+    """element strides of rows of 64 adjacent values; a dimension of one element has none"""
+    st = t.stride()
+    if t.is_contiguous():
+        return st[:-1] if 1 not in t.shape else [v if v % 64 == 0 else 0 for v in st[:-1]]      # (a size-1 dimension's stride is arbitrary)
+    if st[-1] != 1:
         raise ValueError("%s: the 64 values of a row are adjacent" % what)
-    return [0 if n == 1 else st for n, st in zip(sizes, t.stride()[:-1])]
+    return [0 if n == 1 else v for n, v in zip(t.shape[:-1], st)]
 
 
 def cache4_put(cache, x, pos=None, n_new=None):
     """Quantise x (f32 | bf16 [n_kv, N, h, L, 64]; one cache: [N, h, L, 64]) into the slots pos + i of `cache`, i < n_new: pos int32 [1] (all
     rows: `state[:1]` of a decoding step) or [N], default 0; n_new int32 [N], default L.  Slots outside the cache are not written."""
     n_kv, N, h, Tmax = cache.shape
-    if x.dim() != cache.codes.dim() or tuple(x.shape[:-2]) != tuple(cache.codes.shape[:-2]) or x.shape[-1] != 64:
-        raise ValueError("cache4_put: x is [.., L, 64] with the cache's leading dimensions %s, got %s" % (tuple(cache.codes.shape[:-2]), tuple(x.shape)))
-    L = x.shape[-2]
-    st = _cache4_strides("cache4_put", x, x.shape[:-1])
-    ps = _cache4_slots("cache4_put", cache, pos, n_new)
-    with _on("cache4_put", cache.codes, x, pos, n_new):
-        if x.numel() == 0:
-            return
-        check(lib().asr_cache4_put(_stream(), _p(x), dtype_code(x), st[0] if len(st) == 4 else 0, *st[-3:], _p(cache.codes), _p(cache.meta), _p(pos), ps,
-                                   _p(n_new), n_kv, N, h, L, Tmax), "asr_cache4_put")
+    xs = tuple(x.shape)
+    if (xs[:-2] if cache.stack else (1,) + xs[:-2]) != (n_kv, N, h) or xs[-1] != 64:
+        raise ValueError("cache4_put: x is [.., L, 64] with the cache's leading dimensions %s, got %s" % (tuple(cache.codes.shape[:-2]), xs))
+    st = _cache4_strides("cache4_put", x)
+    ps = _cache4_slots("cache4_put", N, pos, n_new)
+    if x.numel() == 0:
+        return
+    _cache4_call("asr_cache4_put", lib().asr_cache4_put, cache, (x, pos, n_new),
+                 (x.data_ptr(), dtype_code(x), st[0] if cache.stack else 0, *st[-3:], cache.codes.data_ptr(), cache.meta.data_ptr(), _ptr(pos), ps, _ptr(n_new), n_kv, N,
+                  h, xs[-2], Tmax))
 
 
 def cache4_get(cache, L=None, pos=None, n_tok=None, dtype=torch.bfloat16):
@@ -1477,40 +1482,49 @@ def cache4_get(cache, L=None, pos=None, n_tok=None, dtype=torch.bfloat16):
     L = Tmax if L is None else int(L)
     if L < 0:
         raise ValueError("cache4_get: L = %d" % L)
-    ps = _cache4_slots("cache4_get", cache, pos, n_tok)
-    with _on("cache4_get", cache.codes, pos, n_tok):
-        out = torch.empty(tuple(cache.codes.shape[:-2]) + (L, 64), device=cache.codes.device, dtype=dtype)
-        code = dtype_code(out)
-        if out.numel():
-            check(lib().asr_cache4_get(_stream(), _p(cache.codes), _p(cache.meta), _p(out), code, N * h * L * 64, h * L * 64, L * 64, 64, _p(pos), ps,
-                                       _p(n_tok), n_kv, N, h, L, Tmax), "asr_cache4_get")
+    ps = _cache4_slots("cache4_get", N, pos, n_tok)
+    out = cache.meta.new_empty((n_kv, N, h, L, 64) if cache.stack else (N, h, L, 64), dtype=dtype)
+    code = dtype_code(out)
+    if out.numel():
+        _cache4_call("asr_cache4_get", lib().asr_cache4_get, cache, (pos, n_tok),
+                     (cache.codes.data_ptr(), cache.meta.data_ptr(), out.data_ptr(), code, N * h * L * 64, h * L * 64, L * 64, 64, _ptr(pos), ps, _ptr(n_tok), n_kv, N, h,
+                      L, Tmax))
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _cache4_workspace(N, h, h_kv, Lq, T, code):
+    return lib().asr_cache4_attention_workspace_bytes(N, h, h_kv, Lq, T, code)      # (a function of the sizes alone)
 
 
 def cache4_attention(q, k_cache, v_cache, k_len=None, causal=False, need_lse=False):
     """attention_fwd over 4-bit caches of N rows (one K, one V: `cache[2 * i]`, `cache[2 * i + 1]`): q [N, h, Lq, 64] (pre-scaled, any strides with
     adjacent rows of 64), h a multiple of the caches' heads -> ctx [N, Lq, h*64] in q's dtype, lse f32 [N, h, Lq] or None.  k_len int32 [N] or
     None; causal: the Lq queries are the last tokens of each row.  A query that sees nothing gets zeros (lse -inf)."""
-    if q.dim() != 4 or q.shape[3] != 64:
-        raise ValueError("cache4_attention: q is [N, h, Lq, 64], got %s" % (tuple(q.shape),))
-    N, h, Lq, _ = q.shape
-    lead = tuple(k_cache.codes.shape)
-    if len(lead) != 4 or tuple(v_cache.codes.shape) != lead or lead[0] != N or lead[1] == 0 or h % lead[1]:
-        raise ValueError("cache4_attention: caches [N, h_kv, T] with N = %d and h_kv dividing %d, got %s and %s" % (N, h, lead[:3], tuple(v_cache.codes.shape[:3])))
-    if k_len is not None and (k_len.dtype != torch.int32 or k_len.numel() != N or not k_len.is_contiguous()):
+    qs = tuple(q.shape)
+    if len(qs) != 4 or qs[3] != 64:
+        raise ValueError("cache4_attention: q is [N, h, Lq, 64], got %s" % (qs,))
+    N, h, Lq, _ = qs
+    _, n, h_kv, T = k_cache.shape
+    if k_cache.stack or v_cache.stack or v_cache.shape != k_cache.shape or n != N or h_kv == 0 or h % h_kv:
+        raise ValueError("cache4_attention: caches [N, h_kv, T] with N = %d and h_kv dividing %d, got %s and %s" %
+                         (N, h, tuple(k_cache.codes.shape[:-1]), tuple(v_cache.codes.shape[:-1])))
+    if k_len is not None and (k_len.dtype is not torch.int32 or k_len.numel() != N or not k_len.is_contiguous()):
         raise ValueError("cache4_attention: k_len is a contiguous int32 tensor of %d elements" % N)
-    h_kv, T, code = lead[1], lead[2], dtype_code(q)
-    st = _cache4_strides("cache4_attention", q, (N, h, Lq))
-    with _on("cache4_attention", q, k_cache.codes, v_cache.codes, k_len):
-        ctx = torch.empty((N, Lq, h * 64), device=q.device, dtype=q.dtype)
-        lse = torch.empty((N, h, Lq), device=q.device, dtype=torch.float32) if need_lse else None
-        if ctx.numel():
-            L = lib()
-            nbytes = L.asr_cache4_attention_workspace_bytes(N, h, h_kv, Lq, T, code)
-            ws = torch.empty(nbytes, device=q.device, dtype=torch.uint8) if nbytes else None
+    code = dtype_code(q)
+    st = _cache4_strides("cache4_attention", q)
+    ctx = q.new_empty((N, Lq, h * 64))
+    lse = q.new_empty((N, h, Lq), dtype=torch.float32) if need_lse else None
+    if N * h * Lq:
+        nbytes = _cache4_workspace(N, h, h_kv, Lq, T, code)
+        ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
+        args = (q.data_ptr(), code, *st, k_cache.codes.data_ptr(), k_cache.meta.data_ptr(), v_cache.codes.data_ptr(), v_cache.meta.data_ptr(), ctx.data_ptr(), _ptr(lse),
+                N, h, h_kv, Lq, T, _ptr(k_len), 1 if causal else 0, _ptr(ws), nbytes)
+        if _PROF is None:
+            _cache4_call("asr_cache4_attention", lib().asr_cache4_attention, k_cache, (q, v_cache.codes, k_len), args)
+        else:
             with _timed("cache4_attention[N%d h%d/%d %dx%d]" % (N, h, h_kv, Lq, T), 4.0 * N * h * 64 * Lq * T):
-                check(L.asr_cache4_attention(_stream(), _p(q), code, *st, _p(k_cache.codes), _p(k_cache.meta), _p(v_cache.codes), _p(v_cache.meta), _p(ctx),
-                                             _p(lse), N, h, h_kv, Lq, T, _p(k_len), 1 if causal else 0, _p(ws), nbytes), "asr_cache4_attention")
+                _cache4_call("asr_cache4_attention", lib().asr_cache4_attention, k_cache, (q, v_cache.codes, k_len), args)
     return ctx, lse
 
 
@@ -1519,21 +1533,20 @@ def cache4_reorder(cache, parent, state, beam, out=None):
     (another cache of the same shape; its positions > state[0] stay as they are)"""
     n_kv, N, h, Tmax = cache.shape
     beam, out = int(beam), cache if out is None else out
-    if out.codes.shape != cache.codes.shape:
+    if out.shape != cache.shape:
         raise ValueError("cache4_reorder: out has the cache's shape")
-    if beam < 1 or N % beam or parent.dtype != torch.int64 or parent.numel() != N or not parent.is_contiguous():
+    if beam < 1 or N % beam or parent.dtype is not torch.int64 or parent.numel() != N or not parent.is_contiguous():
         raise ValueError("cache4_reorder: parent is a contiguous int64 tensor of the cache's %d rows, a multiple of beam = %d" % (N, beam))
-    if state.dtype != torch.int32 or state.numel() < 1 or not state.is_contiguous():
+    if state.dtype is not torch.int32 or state.numel() < 1 or not state.is_contiguous():
         raise ValueError("cache4_reorder: state is a contiguous int32 tensor, the position first")
-    if out is not cache:
-        lo, hi = cache.codes.data_ptr(), cache.codes.data_ptr() + cache.codes.numel()
-        same = out.codes.data_ptr() == lo and out.meta.data_ptr() == cache.meta.data_ptr()
-        if not same and out.codes.data_ptr() < hi and lo < out.codes.data_ptr() + out.codes.numel():
-            raise ValueError("cache4_reorder: out overlaps the cache")
-    with _on("cache4_reorder", cache.codes, out.codes, parent, state):
-        if cache.codes.numel():
-            check(lib().asr_cache4_reorder(_stream(), _p(cache.codes), _p(cache.meta), _p(out.codes), _p(out.meta), _p(parent), _p(state), n_kv, N // beam, beam,
-                                           h, Tmax), "asr_cache4_reorder")
+    src, dst = (cache.codes.data_ptr(), cache.meta.data_ptr()), (out.codes.data_ptr(), out.meta.data_ptr())
+    if src != dst:
+        for a, b, n in zip(src, dst, (n_kv * N * h * Tmax * 32, n_kv * N * h * Tmax * 4)):
+            if a < b + n and b < a + n:
+                raise ValueError("cache4_reorder: out overlaps the cache")
+    if n_kv * N * h * Tmax:
+        _cache4_call("asr_cache4_reorder", lib().asr_cache4_reorder, cache, (out.codes, parent, state), (*src, *dst, parent.data_ptr(), state.data_ptr(), n_kv, N // beam,
+                                                                                                         beam, h, Tmax))
 
 
 def log_softmax_rows(x2d):

@@ -14,7 +14,7 @@ from asr_amd import ops
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 LOG2E = 1.4426950408889634
-UNIT = {torch.bfloat16: 127 * 128, torch.float32: 127 * 16384}      # what the largest element becomes in digits of base 128
+UNIT = {torch.bfloat16: 127 * 256, torch.float32: 127 * 65536}      # what the largest element becomes in digits of base 256
 
 
 def i32(*v):
