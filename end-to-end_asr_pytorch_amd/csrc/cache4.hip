@@ -18,17 +18,27 @@ __device__ __forceinline__ float meta_scale(uint32_t m) { return __builtin_bit_c
 __device__ __forceinline__ float meta_mid(uint32_t m) { return __builtin_bit_cast(float, m & 0xffff0000u); }
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
 
-// ---- 8 consecutive values of a row ---------------------------------------------------------------------------------------------------
-__device__ __forceinline__ void load8(const bf16_t* p, float (&v)[8]) {
-    const u32x4 w = *reinterpret_cast<const u32x4*>(p);
+// ---- 16 consecutive values of a row ---------------------------------------------------------------------------------------------------
+template <typename T> struct Row16;
+template <> struct Row16<bf16_t> {
+    u32x4 w[2];
+    __device__ __forceinline__ void load(const bf16_t* p) { w[0] = reinterpret_cast<const u32x4*>(p)[0]; w[1] = reinterpret_cast<const u32x4*>(p)[1]; }
+    __device__ __forceinline__ void widen(float (&v)[16]) const {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[2 * i] = meta_scale(w[i]); v[2 * i + 1] = meta_mid(w[i]); }
-}
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(p), b = *reinterpret_cast<const f32x4*>(p + 4);
+        for (int i = 0; i < 8; ++i) { v[2 * i] = meta_scale(w[i >> 2][i & 3]); v[2 * i + 1] = meta_mid(w[i >> 2][i & 3]); }
+    }
+};
+template <> struct Row16<float> {
+    f32x4 w[4];
+    __device__ __forceinline__ void load(const float* p) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
-}
+        for (int i = 0; i < 4; ++i) w[i] = reinterpret_cast<const f32x4*>(p)[i];
+    }
+    __device__ __forceinline__ void widen(float (&v)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = w[i >> 2][i & 3];
+    }
+};
 __device__ __forceinline__ void store8(bf16_t* p, const float (&v)[8]) {
     bf16x8 o;
 #pragma unroll
@@ -42,11 +52,6 @@ __device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
 
 template <int CTRL> __device__ __forceinline__ float dpp_f(float x) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xf, 0xf, true));
-}
-template <int CTRL> __device__ __forceinline__ void minmax_step(float& lo, float& hi, float& bad) {
-    lo = fminf(lo, dpp_f<CTRL>(lo));
-    hi = fmaxf(hi, dpp_f<CTRL>(hi));
-    bad += dpp_f<CTRL>(bad);
 }
 // d / s with one correction: the quotient rounded to nearest (where it has few bits - on a border k + 1/2 - exactly that), rs = 1 / s to an ulp or two
 __device__ __forceinline__ float quotient(float d, float s, float rs) {
@@ -64,112 +69,132 @@ __device__ __forceinline__ float quotient(float d, float s, float rs) {
 // (Exact for all of them, with the rounding error of the subtraction carried along, is 12 instructions a value more: VALU-bound.)
 template <typename T> __device__ __forceinline__ u32x2 quantise16(const float (&x)[16], uint32_t& meta) {
 #pragma clang fp contract(off)
-    float lo = x[0], hi = x[0], bad = 0.f;      // bad: 0, or NaN where a value is not finite
+    float lo = x[0], hi = x[0];      // (v_minimum3 / v_maximum3: a NaN stays, an infinity is an extreme - span is finite only if every value is)
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        bad = __builtin_fmaf(x[i], 0.f, bad);
+    for (int i = 1; i < 16; ++i) {
+        lo = __builtin_elementwise_minimum(lo, x[i]);
+        hi = __builtin_elementwise_maximum(hi, x[i]);
     }
-    minmax_step<0xB1>(lo, hi, bad);      // quad_perm: lane xor 1, lane xor 2
-    minmax_step<0x4E>(lo, hi, bad);
-    const float span = (hi - lo) + bad;
+    lo = __builtin_elementwise_minimum(lo, dpp_f<0xB1>(lo));      // quad_perm: lane xor 1, lane xor 2
+    hi = __builtin_elementwise_maximum(hi, dpp_f<0xB1>(hi));
+    lo = __builtin_elementwise_minimum(lo, dpp_f<0x4E>(lo));
+    hi = __builtin_elementwise_maximum(hi, dpp_f<0x4E>(hi));
+    const float span = hi - lo;
     const bool fine = span < INFINITY;
-    const float sc = span < 0x1p-100f || !fine ? 0.f : (float)(bf16_t)(span / 15.f);
+    // (span / 15 rounded to nearest: 1.f / 15.f is the reciprocal rounded to nearest, so one corrected step is the correctly rounded quotient)
+    const float sc = span < 0x1p-100f || !fine ? 0.f : (float)(bf16_t)quotient(span, 15.f, 1.f / 15.f);
     const float mid = (float)(bf16_t)(lo + 8.f * sc);
     meta = fine ? bf16_bits(sc) | (bf16_bits(mid) << 16) : 0x7fc07fc0u;
     if (sc == 0.f) return u32x2{0u, 0u};
     const float rs = __builtin_amdgcn_rcpf(sc);
-    float k[16], near = 0.f;
+    constexpr float MAGIC = 12582912.f + 8.f;      // 1.5 * 2^23: adding it rounds to the nearest integer, ties to even, and leaves code + 8 in the low bits
+    float y[16], near = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
-        const float y = quotient(x[i] - mid, sc, rs);
-        k[i] = __builtin_rintf(y);
-        if (sizeof(T) == 4) near = fmaxf(near, fabsf(y - k[i]));
+        y[i] = quotient(x[i] - mid, sc, rs);
+        if (sizeof(T) == 4) near = fmaxf(near, fabsf(y[i] - __builtin_rintf(y[i])));
+        y[i] = __builtin_amdgcn_fmed3f(y[i], -8.f, 7.f);
     }
     bool again = near > 0.5f - 0x1p-19f;
     if (sizeof(T) == 2) {
-        const float ym = quotient(mid, sc, rs);
-        again = __builtin_rintf(2.f * ym) == 2.f * ym && __builtin_rintf(ym) != ym;
+        const float ym = 2.f * quotient(mid, sc, rs);
+        again = __builtin_rintf(ym) == ym && __builtin_rintf(0.5f * ym) != 0.5f * ym;
     }
     if (__builtin_expect(again, 0)) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const float d = x[i] - mid, bb = d - x[i], e = (x[i] - (d - bb)) + (-mid - bb);      // d + e = x - mid exactly
-            const float r = __builtin_fmaf(-k[i], sc, d);                                        // exact next to a border: k sc has 12 bits
+            const float k = __builtin_rintf(y[i]), r = __builtin_fmaf(-k, sc, d);                // exact next to a border: k sc has 12 bits
             const float g = (fabsf(r) - 0.5f * sc) + (r > 0.f ? e : -e);                         // > 0: the neighbour is nearer
-            const bool move = (g > 0.f) | ((g == 0.f) & (((int)k[i] & 1) != 0));
-            k[i] += move ? __builtin_copysignf(1.f, r) : 0.f;
+            const bool move = (g > 0.f) | ((g == 0.f) & (((int)k & 1) != 0));
+            y[i] = __builtin_amdgcn_fmed3f(move ? k + __builtin_copysignf(1.f, r) : k, -8.f, 7.f);
         }
     }
-    u32x2 w = {0u, 0u};
+    u32x2 w;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) w[i >> 3] |= (uint32_t)(int)(__builtin_amdgcn_fmed3f(k[i], -8.f, 7.f) + 8.f) << (4 * (i & 7));
+    for (int j = 0; j < 2; ++j) {
+        uint32_t p[4];      // the low byte: two codes
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            p[i] = __builtin_bit_cast(uint32_t, y[8 * j + 2 * i] + MAGIC) | (__builtin_bit_cast(uint32_t, y[8 * j + 2 * i + 1] + MAGIC) << 4);
+        w[j] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(p[3], p[2], 0x0c0c0400u), __builtin_amdgcn_perm(p[1], p[0], 0x0c0c0400u), 0x05040100u);
+    }
     return w ^ 0x88888888u;      // offset code -> two's complement nibble
 }
 
-// Slots of one call: which rows a block works on.  A block is 256 / LANES groups of LANES lanes, one row of 64 values each; `tb` (a power of
-// two) tokens of as many rows as fill the block side by side, so that a single token per row fills it as well as a long chunk does; a long
-// chunk's block walks ITER * tb tokens.
-constexpr int ITER = 4;
+// Slots of one call: which rows a block works on.  A block is 256 / LANES groups of LANES lanes, one row of 64 values each; 2^tb_log2 tokens
+// of as many rows as fill the block side by side, so that a single token per row fills it as well as a long chunk does.  A long chunk's
+// block belongs to one row (ONE_ROW: its addresses are scalar) and walks `iter` times its width.
 struct slots_t {
     const int32_t* pos; const int32_t* n_tok;
-    int pos_stride, N, h, L, Tmax, tb_log2, rb_log2, chunks, rows;
+    int pos_stride, N, h, L, Tmax, tb_log2, rb_log2, iter, chunks, rows;
 };
 struct strides_t { int64_t kv, n, head, tok; };
+struct range_t { int64_t x0, c0; int i, end, step, lo, hi; };      // tokens i, i + step, .. < end; those of [lo, hi) have a slot: c0 + token
 
-template <int LANES, typename F> __device__ __forceinline__ void for_tokens(const slots_t& s, const strides_t& st, F f) {
+template <int LANES, bool ONE_ROW> __device__ __forceinline__ bool range_of(const slots_t& s, const strides_t& st, range_t& r) {
     const int chunk = s.chunks == 1 ? 0 : blockIdx.x % s.chunks, rows = s.chunks == 1 ? blockIdx.x : blockIdx.x / s.chunks, group = threadIdx.x / LANES;
-    const int row = (rows << s.rb_log2) + (group >> s.tb_log2);
-    if (row >= s.rows) return;
+    const int row = ONE_ROW ? rows : (rows << s.rb_log2) + (group >> s.tb_log2);
+    if (row >= s.rows) return false;
     const int head = row % s.h, kn = row / s.h, n = kn % s.N, kv = kn / s.N;
-    const int first = s.pos ? s.pos[(int64_t)n * s.pos_stride] : 0;
+    const int64_t first = s.pos ? s.pos[(int64_t)n * s.pos_stride] : 0, room = (int64_t)s.Tmax - first;
     const int count = s.n_tok ? clampi(s.n_tok[n], 0, s.L) : s.L;
-    const int64_t x0 = kv * st.kv + n * st.n + head * st.head;
-    const int64_t c0 = (int64_t)row * s.Tmax;
-    const int tb = 1 << s.tb_log2, t0 = chunk * (tb * ITER) + (group & (tb - 1));
-#pragma unroll 1
-    for (int it = 0; it < ITER; ++it) {
-        const int i = t0 + it * tb;
-        if (i >= s.L) break;
-        f(i, count, first, x0 + (int64_t)i * st.tok, c0);
+    r.lo = first < 0 ? (int)(-first < s.L ? -first : s.L) : 0;
+    r.hi = (int)(room < count ? (room > 0 ? room : 0) : count);
+    r.x0 = kv * st.kv + n * st.n + head * st.head;
+    r.c0 = (int64_t)row * s.Tmax + first;
+    r.step = 1 << s.tb_log2;
+    const int t0 = chunk * (s.iter << s.tb_log2);
+    r.i = t0 + (group & (r.step - 1));
+    r.end = min(t0 + (s.iter << s.tb_log2), s.L);
+    return true;
+}
+
+template <typename T, bool ONE_ROW>
+__global__ __launch_bounds__(256) void cache4_put_kernel(const T* __restrict__ x, strides_t st, uint32_t* __restrict__ codes,
+                                                         uint32_t* __restrict__ meta, slots_t s) {
+    range_t r;
+    if (!range_of<4, ONE_ROW>(s, st, r)) return;
+    const int l4 = threadIdx.x & 3, end = min(r.end, r.hi);
+    const T* px = x + r.x0 + l4 * 16;
+    uint32_t* pc = codes + r.c0 * 8 + l4 * 2;
+    uint32_t* pm = meta + r.c0;
+    int i = r.i;
+    if (i < r.lo) i += (r.lo - i + r.step - 1) & ~(r.step - 1);
+    if (i >= end) return;      // (one token's 4 lanes agree, here and below)
+    Row16<T> w;
+    w.load(px + (int64_t)i * st.tok);
+    for (; i < end; i += r.step) {
+        float v[16];
+        w.widen(v);
+        if (i + r.step < end) w.load(px + (int64_t)(i + r.step) * st.tok);      // the next row's while this one is worked on
+        uint32_t m;
+        const u32x2 c = quantise16<T>(v, m);
+        *reinterpret_cast<u32x2*>(pc + (unsigned)i * 8u) = c;
+        if (l4 == 0) pm[(unsigned)i] = m;
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void cache4_put_kernel(const T* __restrict__ x, strides_t st, uint32_t* __restrict__ codes,
-                                                         uint32_t* __restrict__ meta, slots_t s) {
-    const int l4 = threadIdx.x & 3;
-    for_tokens<4>(s, st, [&](int i, int count, int first, int64_t xo, int64_t c0) {
-        const int64_t slot = (int64_t)first + i;
-        if (i >= count || slot < 0 || slot >= s.Tmax) return;      // (one token's 4 lanes agree)
-        float v[16], a[8], b[8];
-        load8(x + xo + l4 * 16, a);
-        load8(x + xo + l4 * 16 + 8, b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) { v[j] = a[j]; v[8 + j] = b[j]; }
-        uint32_t m;
-        const u32x2 w = quantise16<T>(v, m);
-        *reinterpret_cast<u32x2*>(codes + (c0 + slot) * 8 + l4 * 2) = w;
-        if (l4 == 0) meta[c0 + slot] = m;
-    });
-}
-
-template <typename T>
+template <typename T, bool ONE_ROW>
 __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, strides_t st, const uint32_t* __restrict__ codes,
                                                          const uint32_t* __restrict__ meta, slots_t s) {
+    range_t r;
+    if (!range_of<8, ONE_ROW>(s, st, r)) return;
     const int l8 = threadIdx.x & 7;
-    for_tokens<8>(s, st, [&](int i, int count, int first, int64_t xo, int64_t c0) {
-        const int64_t slot = (int64_t)first + i;
+    T* po = out + r.x0 + l8 * 8;
+    const uint32_t* pc = codes + r.c0 * 8 + l8;
+    const uint32_t* pm = meta + r.c0;
+#pragma unroll 2
+    for (int i = r.i; i < r.end; i += r.step) {
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        if (i < count && slot >= 0 && slot < s.Tmax) {
-            const uint32_t w = codes[(c0 + slot) * 8 + l8], m = meta[c0 + slot];
+        if (i >= r.lo && i < r.hi) {
+            const uint32_t w = pc[(unsigned)i * 8u], m = pm[(unsigned)i];
             const float sc = meta_scale(m), mid = meta_mid(m);
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] = __builtin_fmaf(sc, (float)((int)(w << (28 - 4 * j)) >> 28), mid);      // one rounding: sc * code is exact
         }
-        store8(out + xo + l8 * 8, v);
-    });
+        store8(po + (int64_t)i * st.tok, v);
+    }
 }
 
 // ---- re-gathering by parent ------------------------------------------------------------------------------------------------------------
@@ -218,8 +243,9 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
 // largest, so a tile of small weights keeps its precision).  ND = 2 digits for bf16 queries (half a step is 2^-16 of the largest, below the
 // 2^-9 that a bf16 weight is rounded by), 3 for f32 (2^-24).  The products are exact int32; softmax statistics and the output are f32.
 //
-// A wave owns 64 tokens at a time, token = lane: the query operand of each of a tile's four QK instructions is zero except in the four rows
-// whose results land in the sixteen lanes of the right tokens, so one accumulator collects 64 tokens x (2 queries x 2 digits, or 1 x 3).
+// A wave owns 64 tokens at a time, token = lane.  A 16-byte load of K is half a token's channels, so the four lane groups of a QK instruction
+// hold the halves of two tokens: the query operand is zero in the rows whose results land with the other token, and an accumulator of 32
+// tokens holds (2 queries x 2 digits, or 1 x 3) a lane.
 // The weights go through LDS (16 bytes per token: all digits of all queries) into the A operand of the PV product - ds_read_b64_tr_b8 turns
 // them into rows (query, digit) - whose B operand, 16 tokens of one channel per lane, is what ds_read_b64_tr_b4 makes of the tile's
 // row-major codes.
@@ -244,6 +270,7 @@ struct attn4_t {
     int N, h, h_kv, Lq, T, splits, qtiles, rows, waves;
 };
 constexpr int PART = 66;      // floats of a partial result: 64 outputs (not divided), reference, sum
+constexpr int MAX_NQ = 4, MAX_WAVES = 8;
 constexpr float NO_REF = -3.4028234663852886e38f;
 
 // position of element k of 16 in the byte order that unpacking leaves: low nibbles of the first word, its high ones, then the second word's
@@ -318,10 +345,10 @@ __device__ __forceinline__ void load_tile(tile4_t& t, const u32x4* kc, const u32
 }
 
 template <typename T, int ND, int NQ, bool CAUSAL>
-__global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
+__global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) {
     using D = Digits<ND>;
-    constexpr int PASSES = (NQ + D::QPP - 1) / D::QPP, SLOTS = NQ > 4 ? 2 : 1;
-    static_assert(ND == 2 ? NQ <= 8 : NQ <= 4, "16 rows of (query, digit)");
+    constexpr int PASSES = (NQ + D::QPP - 1) / D::QPP;
+    static_assert(NQ <= MAX_NQ, "the rows of lane group c are query c's digits");
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = a.waves, n16 = lane & 15, c = lane >> 4;
     // block -> (row, query tile, split): the query tiles of one stream of keys follow each other at a distance of 8 blocks (one XCD's L2)
@@ -364,20 +391,18 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
         if (lane == 0) { sm_qs[2 * j] = unit; sm_qs[2 * j + 1] = some ? sum / unit : 0.f; }
     }
     __syncthreads();
-    i32x4 qa[PASSES][2][2];      // [j]: tokens 32 j .. 32 j + 31 of the tile, [half]: the first or second 16 of a lane's 32 channels
+    i32x4 qa[PASSES][2];      // [half]: the first or second 16 of a lane's 32 channels
 #pragma unroll
     for (int p = 0; p < PASSES; ++p) {
         const int r = n16 & 3, q = D::QPP == 2 ? 2 * p + (r >> 1) : p, d = D::QPP == 2 ? r & 1 : r;
+        const bool on = ((n16 >> 2) & 1) == (c >> 1) && q < NQ && d < ND;
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const bool on = (n16 >> 2) == 2 * j + (c >> 1) && q < NQ && d < ND;
-                const i32x4 v = *reinterpret_cast<const i32x4*>(sm_q + (min(q, NQ - 1) * ND + min(d, ND - 1)) * 64 + (2 * (c & 1) + half) * 16);
-                qa[p][j][half] = on ? v : i32x4{0, 0, 0, 0};
-            }
+        for (int half = 0; half < 2; ++half) {
+            const i32x4 v = *reinterpret_cast<const i32x4*>(sm_q + (min(q, NQ - 1) * ND + min(d, ND - 1)) * 64 + (2 * (c & 1) + half) * 16);
+            qa[p][half] = on ? v : i32x4{0, 0, 0, 0};
+        }
     }
-    float unit[NQ], qsum[NQ], m[NQ], l[NQ], mv[NQ], acc[4][SLOTS];
+    float unit[NQ], qsum[NQ], m[NQ], l[NQ], mv[NQ], acc[4];
     int lim[NQ];      // first token that the query does not see
 #pragma unroll
     for (int q = 0; q < NQ; ++q) {
@@ -386,9 +411,7 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
         lim[q] = CAUSAL ? klen - (a.Lq - 1) + (q0 + q) % a.Lq : klen;
     }
 #pragma unroll
-    for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int s = 0; s < SLOTS; ++s) acc[d][s] = 0.f;
+    for (int d = 0; d < 4; ++d) acc[d] = 0.f;
 
     const int step = a.splits * W;
     for (; tile < tiles; tile += step) {
@@ -409,14 +432,16 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
         float s[NQ], e[NQ], top = -INFINITY;
 #pragma unroll
         for (int p = 0; p < PASSES; ++p) {
-            i32x4 dot = {0, 0, 0, 0};
+            i32x4 dot[2];      // [j]: rows of the lanes 32 j .. 32 j + 31
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) dot = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[p][j][half], ku[j][half], dot, 0, 0, 0);
+            for (int j = 0; j < 2; ++j) {
+                dot[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[p][0], ku[j][0], i32x4{0, 0, 0, 0}, 0, 0, 0);
+                dot[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(qa[p][1], ku[j][1], dot[j], 0, 0, 0);
+            }
+            const i32x4 d = {lane < 32 ? dot[0][0] : dot[1][0], lane < 32 ? dot[0][1] : dot[1][1], lane < 32 ? dot[0][2] : dot[1][2], lane < 32 ? dot[0][3] : dot[1][3]};
 #pragma unroll
             for (int i = 0; i < D::QPP; ++i)
-                if (D::QPP * p + i < NQ) s[D::QPP * p + i] = D::QPP == 2 ? D::join(dot[2 * i], dot[2 * i + 1], 0) : D::join(dot[0], dot[1], dot[2]);
+                if (D::QPP * p + i < NQ) s[D::QPP * p + i] = D::QPP == 2 ? D::join(d[2 * i], d[2 * i + 1], 0) : D::join(d[0], d[1], d[2]);
         }
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
@@ -434,54 +459,39 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
                 m[q] = mn; l[q] *= al[q]; mv[q] *= al[q];
                 e[q] = __builtin_fmaf(s[q], unit[q], -mn);
             }
+            float f = 1.f;
 #pragma unroll
-            for (int sl = 0; sl < SLOTS; ++sl) {
-                float f = 1.f;
+            for (int q = 0; q < NQ; ++q) f = c == q ? al[q] : f;
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    if (4 * sl + q < NQ && c == q) f = al[4 * sl + q < NQ ? 4 * sl + q : 0];
-#pragma unroll
-                for (int d = 0; d < 4; ++d) acc[d][sl] *= f;
-            }
+            for (int d = 0; d < 4; ++d) acc[d] *= f;
         }
         // weights -> digits
-        float w[4 * SLOTS], wunit[SLOTS], inv[SLOTS];
-        uint32_t u[4 * SLOTS];
+        float w[MAX_NQ];
+        uint32_t u[MAX_NQ];
 #pragma unroll
-        for (int q = 0; q < 4 * SLOTS; ++q) {
+        for (int q = 0; q < MAX_NQ; ++q) {
             w[q] = 0.f;
-            if (q < NQ) {
-                const float p = __builtin_amdgcn_exp2f(e[q < NQ ? q : 0]);
-                const bool seen = !CAUSAL || tok < lim[q < NQ ? q : 0];      // (0 * NaN of a token that another query sees must not enter the sums)
-                l[q < NQ ? q : 0] += p;
-                mv[q < NQ ? q : 0] = __builtin_fmaf(p, seen ? vmid : 0.f, mv[q < NQ ? q : 0]);
-                w[q] = p * (seen ? vsc : 0.f);
-            }
+            u[q] = 0u;
+            if (q >= NQ) continue;
+            const float p = __builtin_amdgcn_exp2f(e[q]);
+            const bool seen = !CAUSAL || tok < lim[q];      // (0 * NaN of a token that another query sees must not enter the sums)
+            l[q] += p;
+            mv[q] = __builtin_fmaf(p, seen ? vmid : 0.f, mv[q]);
+            w[q] = p * (seen ? vsc : 0.f);
         }
-#pragma unroll
-        for (int sl = 0; sl < SLOTS; ++sl) {
-            const float most = NQ == 1 ? wave_all<MaxPos>(w[0]) : wave_four<MaxPos>(w[4 * sl], w[4 * sl + 1], w[4 * sl + 2], w[4 * sl + 3]);      // of query 4 sl + c
-            inv[sl] = most > 1e-30f ? D::UNIT * __builtin_amdgcn_rcpf(most) : 0.f;
-            wunit[sl] = most * (1.f / (16.f * D::UNIT));
-        }
+        const float most = NQ == 1 ? wave_all<MaxPos>(w[0]) : wave_four<MaxPos>(w[0], w[1], w[2], w[3]);      // of query c
+        const float inv = most > 1e-30f ? D::UNIT * __builtin_amdgcn_rcpf(most) : 0.f, wunit = most * (1.f / (16.f * D::UNIT));
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
-            const float iq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv[q >> 2]), 16 * (q & 3)));
+            const float iq = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, inv), 16 * q));
             if (ND == 2) u[q] = __builtin_bit_cast(uint32_t, __builtin_fmaf(w[q], iq, 12582912.f + D::BIAS));      // round to nearest: the integer in the low bits
-            else u[q] = (uint32_t)__builtin_fmaf(w[q], iq, D::BIAS + 0.5f) ^ D::BIAS;
-        }
-        uint32_t pw[4];
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            pw[q] = 0u;
-            if (q < NQ) pw[q] = u[q < NQ ? q : 0];
-            if (ND == 2 && q + 4 < NQ) pw[q] = __builtin_amdgcn_perm(u[q + 4 < NQ ? q + 4 : 0], pw[q], 0x05040100u);
-            if (ND == 2) pw[q] ^= 0x00800080u;
+            else u[q] = (uint32_t)__builtin_fmaf(w[q], iq, D::BIAS + 0.5f);
+            u[q] ^= D::BIAS;
         }
         unsigned char* to = sm_p + ((lane & 48) + unpack_pos(n16)) * 16;
-        if (NQ == 1) *reinterpret_cast<uint32_t*>(to) = pw[0];
-        else if (NQ == 2) *reinterpret_cast<u32x2*>(to) = u32x2{pw[0], pw[1]};
-        else *reinterpret_cast<u32x4*>(to) = u32x4{pw[0], pw[1], pw[2], pw[3]};
+        if (NQ == 1) *reinterpret_cast<uint32_t*>(to) = u[0];
+        else if (NQ == 2) *reinterpret_cast<u32x2*>(to) = u32x2{u[0], u[1]};
+        else *reinterpret_cast<u32x4*>(to) = u32x4{u[0], u[1], u[2], u[3]};
         wave_lds_fence();
         lds_i32x2* from = (lds_i32x2*)((__attribute__((address_space(3))) unsigned char*)sm_p + c * 256 + n16 * 8);
         const i32x2 p0 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(from), p1 = __builtin_amdgcn_ds_read_tr8_b64_v2i32(from + 16);
@@ -491,8 +501,7 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
             const i32x2 vt = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)((__attribute__((address_space(3))) unsigned char*)sm_v + lane * 32 +
                                                                                   (((d >> 1) ^ ((lane >> 3) & 1)) << 4) + (d & 1) * 8));
             const i32x4 o = __builtin_amdgcn_mfma_i32_16x16x64_i8(pa, unpack16((uint32_t)vt[0], (uint32_t)vt[1]), i32x4{0, 0, 0, 0}, 0, 0, 0);
-            acc[d][0] = __builtin_fmaf(D::join(o[0], o[1], o[2]), wunit[0], acc[d][0]);
-            if (SLOTS == 2) acc[d][SLOTS - 1] = __builtin_fmaf(D::join(o[2], o[3], 0), wunit[SLOTS - 1], acc[d][SLOTS - 1]);
+            acc[d] = __builtin_fmaf(D::join(o[0], o[1], o[2]), wunit, acc[d]);
         }
         wave_lds_fence();
     }
@@ -505,9 +514,9 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
     for (int q = 0; q < NQ; ++q) {
         const float lw = wave_all<SumF>(l[q]), mw = wave_all<SumF>(mv[q]);
         if (lane == 0) { sm_m[(wave * NQ + q) * 2] = m[q]; sm_m[(wave * NQ + q) * 2 + 1] = lw; }
-        if (c == (q & 3))
+        if (c == q)
 #pragma unroll
-            for (int d = 0; d < 4; ++d) sm_o[(wave * NQ + q) * 64 + d * 16 + n16] = acc[d][q >> 2] + mw;
+            for (int d = 0; d < 4; ++d) sm_o[(wave * NQ + q) * 64 + d * 16 + n16] = acc[d] + mw;
     }
     __syncthreads();
     for (int q = wave; q < nq; q += W) {
@@ -530,54 +539,65 @@ __global__ __launch_bounds__(512) void cache4_attn_kernel(attn4_t a) {
     }
 }
 
-// joins the splits of one query: 4 waves take every fourth partial result
+// joins the splits of one query: 8 waves of up to MAX_SPLITS / 8 partial results each, all loads in front
+constexpr int MAX_SPLITS = 32, JOIN_WAVES = 8;
 template <typename T>
-__global__ __launch_bounds__(256) void cache4_join_kernel(attn4_t a) {
-    __shared__ float sm[4][PART];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = a.h / a.h_kv, Q = group * a.Lq;
-    const int row = blockIdx.x / Q, qi = blockIdx.x % Q, n = row / a.h_kv, hk = row % a.h_kv;
-    const int klen = a.k_len ? clampi(a.k_len[n], 0, a.T) : a.T, live = clampi(((klen + 63) / 64 + a.waves - 1) / a.waves, 1, a.splits);
+__global__ __launch_bounds__(JOIN_WAVES * 64) void cache4_join_kernel(attn4_t a) {
+    __shared__ float sm[JOIN_WAVES][PART];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = a.h / a.h_kv, Q = group * a.Lq;
+    const int row = blockIdx.x / Q, qi = blockIdx.x - row * Q, n = row / a.h_kv, hk = row - n * a.h_kv;
     const float* part = a.part + ((int64_t)row * Q + qi) * a.splits * PART;
+    constexpr int MINE = MAX_SPLITS / JOIN_WAVES;
+    float v[MINE], ms[MINE], ls[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {      // (inside the workspace also where a split had no tile and left nothing: not used below)
+        const float* p = part + (int64_t)min(wave + i * JOIN_WAVES, a.splits - 1) * PART;
+        v[i] = p[lane]; ms[i] = p[64]; ls[i] = p[65];
+    }
+    const int klen = a.k_len ? clampi(a.k_len[n], 0, a.T) : a.T, live = clampi(((klen + 63) / 64 + a.waves - 1) / a.waves, 1, a.splits);
     float M = NO_REF, L = 0.f, o = 0.f;
-    for (int s = wave; s < live; s += 4) {
-        const float* p = part + (int64_t)s * PART;
-        const float v = p[lane], ms = p[64], ls = p[65], mn = fmaxf(M, ms);
-        const float f0 = __builtin_amdgcn_exp2f(M - mn), f1 = __builtin_amdgcn_exp2f(ms - mn);
-        L = __builtin_fmaf(ls, f1, L * f0);
-        o = __builtin_fmaf(v, f1, o * f0);
-        M = mn;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) M = wave + i * JOIN_WAVES < live ? fmaxf(M, ms[i]) : M;
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        if (wave + i * JOIN_WAVES >= live) continue;
+        const float f = __builtin_amdgcn_exp2f(ms[i] - M);
+        L = __builtin_fmaf(ls[i], f, L);
+        o = __builtin_fmaf(v[i], f, o);
     }
     sm[wave][lane] = o;
     if (lane == 0) { sm[wave][64] = M; sm[wave][65] = L; }
     __syncthreads();
     if (wave) return;
-    M = fmaxf(fmaxf(sm[0][64], sm[1][64]), fmaxf(sm[2][64], sm[3][64]));
     L = 0.f; o = 0.f;
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
+    for (int w = 0; w < JOIN_WAVES; ++w) M = fmaxf(M, sm[w][64]);
+#pragma unroll
+    for (int w = 0; w < JOIN_WAVES; ++w) {
         const float f = __builtin_amdgcn_exp2f(sm[w][64] - M);
         L = __builtin_fmaf(sm[w][65], f, L);
         o = __builtin_fmaf(sm[w][lane], f, o);
     }
-    const int head = hk * group + qi / a.Lq, i = qi % a.Lq;
+    const int g = qi / a.Lq, head = hk * group + g, i = qi - g * a.Lq;
     static_cast<T*>(a.ctx)[(((int64_t)n * a.Lq + i) * a.h + head) * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : o / L);
     if (a.lse && lane == 0) a.lse[((int64_t)n * a.h + head) * a.Lq + i] = L == 0.f ? -INFINITY : M + __log2f(L);
 }
 
 // How a call is cut: queries per block, splits of the keys.
 struct plan_t { int nq, qtiles, splits, waves; };
-plan_t attn_plan(int rows, int Q, int T, int dtype) {
+plan_t attn_plan(int rows, int Q, int T) {
     plan_t p;
-    const int most = dtype == ASR_BF16 ? 8 : 4;
-    p.qtiles = (Q + most - 1) / most;
+    p.qtiles = (Q + MAX_NQ - 1) / MAX_NQ;
     p.nq = (Q + p.qtiles - 1) / p.qtiles;
     const int tiles = (T + 63) / 64;
-    p.waves = tiles < 8 ? (tiles < 4 ? (tiles < 2 ? 1 : 2) : 4) : 8;
     const int64_t blocks = (int64_t)rows * p.qtiles;
+    const int most = blocks >= 512 ? 4 : 8;
+    p.waves = 1;
+    while (p.waves < most && p.waves < tiles) p.waves *= 2;
     p.splits = 1;
-    if (tiles > 8 && blocks < 512) {
-        const int64_t want = (512 + blocks - 1) / blocks, most_splits = (tiles + 15) / 16;
-        p.splits = (int)(want < most_splits ? want : most_splits);
+    if (tiles > 32 && blocks <= 128) {
+        const int64_t room = 256 / blocks, work = (tiles + 15) / 16, cap = MAX_SPLITS;
+        p.splits = (int)(room < work ? (room < cap ? room : cap) : (work < cap ? work : cap));
     }
     return p;
 }
@@ -589,16 +609,14 @@ template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, c
     const dim3 grid((unsigned)(a.qtiles == 1 ? streams : (streams + 7) / 8 * 8 * a.qtiles)), block(p.waves * 64);
 #define ASR_C4(NQ)                                                                                      \
     case NQ:                                                                                            \
-        if constexpr (ND == 2 || NQ <= 4) {                                                             \
-            if (causal) hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, true>), grid, block, lds, s, a); \
-            else hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, false>), grid, block, lds, s, a);    \
-        }                                                                                               \
+        if (causal) hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, true>), grid, block, lds, s, a);  \
+        else hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, false>), grid, block, lds, s, a);        \
         break;
-    switch (p.nq) { ASR_C4(1) ASR_C4(2) ASR_C4(3) ASR_C4(4) ASR_C4(5) ASR_C4(6) ASR_C4(7) ASR_C4(8) }
+    switch (p.nq) { ASR_C4(1) ASR_C4(2) ASR_C4(3) ASR_C4(4) }
 #undef ASR_C4
     ASR_LAUNCH_CHECK("cache4_attention");
     if (a.splits > 1) {
-        hipLaunchKernelGGL((cache4_join_kernel<T>), dim3((unsigned)((int64_t)a.rows * (a.h / a.h_kv) * a.Lq)), dim3(256), 0, s, a);
+        hipLaunchKernelGGL((cache4_join_kernel<T>), dim3((unsigned)((int64_t)a.rows * (a.h / a.h_kv) * a.Lq)), dim3(JOIN_WAVES * 64), 0, s, a);
         ASR_LAUNCH_CHECK("cache4_attention (join)");
     }
     return 0;
@@ -613,10 +631,10 @@ int slots_plan(const char* name, int lanes, slots_t& s, int64_t& blocks, int n_k
     const int groups_log2 = lanes == 4 ? 6 : 5;      // rows of 64 values side by side in a block of 256 threads
     int lg = 0;
     while (lg < groups_log2 && (1 << lg) < L) ++lg;
-    const int rb_log2 = groups_log2 - lg, chunks = (int)((L + ((int64_t)ITER << lg) - 1) / ((int64_t)ITER << lg));
+    const int rb_log2 = groups_log2 - lg, iter = 4, chunks = (int)((L + ((int64_t)iter << lg) - 1) / ((int64_t)iter << lg));
     blocks = (rows + (1 << rb_log2) - 1) / (1 << rb_log2) * chunks;
     ASR_REQUIRE(rows <= INT32_MAX - 64 && blocks <= INT32_MAX, ASR_ERR_UNSUPPORTED, "%s: too many rows", name);
-    s = slots_t{pos, n_tok, pos_stride, N, h, L, Tmax, lg, rb_log2, chunks, (int)rows};
+    s = slots_t{pos, n_tok, pos_stride, N, h, L, Tmax, lg, rb_log2, iter, chunks, (int)rows};
     return 0;
 }
 bool strides_ok(const strides_t& st, int per16) { return st.kv % per16 == 0 && st.n % per16 == 0 && st.head % per16 == 0 && st.tok % per16 == 0; }
@@ -633,12 +651,13 @@ extern "C" int asr_cache4_put(void* stream, const void* x, int x_dtype, int64_t 
     ASR_REQUIRE(asr_aligned(x, 16) && asr_aligned(codes, 16) && asr_aligned(meta, 4) && strides_ok(st, x_dtype == ASR_F32 ? 4 : 8), ASR_ERR_ALIGN,
                 "cache4_put: rows of x start on 16 bytes, codes on 16, meta on 4");
     hipStream_t hs = static_cast<hipStream_t>(stream);
-    if (x_dtype == ASR_F32)
-        hipLaunchKernelGGL((cache4_put_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const float*>(x), st,
-                           static_cast<uint32_t*>(codes), static_cast<uint32_t*>(meta), s);
-    else
-        hipLaunchKernelGGL((cache4_put_kernel<bf16_t>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const bf16_t*>(x), st,
-                           static_cast<uint32_t*>(codes), static_cast<uint32_t*>(meta), s);
+    if (x_dtype == ASR_F32) {
+        if (s.rb_log2 == 0) hipLaunchKernelGGL((cache4_put_kernel<float, true>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const float*>(x), st, static_cast<uint32_t*>(codes), static_cast<uint32_t*>(meta), s);
+        else hipLaunchKernelGGL((cache4_put_kernel<float, false>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const float*>(x), st, static_cast<uint32_t*>(codes), static_cast<uint32_t*>(meta), s);
+    } else {
+        if (s.rb_log2 == 0) hipLaunchKernelGGL((cache4_put_kernel<bf16_t, true>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const bf16_t*>(x), st, static_cast<uint32_t*>(codes), static_cast<uint32_t*>(meta), s);
+        else hipLaunchKernelGGL((cache4_put_kernel<bf16_t, false>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const bf16_t*>(x), st, static_cast<uint32_t*>(codes), static_cast<uint32_t*>(meta), s);
+    }
     ASR_LAUNCH_CHECK("cache4_put");
     return 0;
 }
@@ -653,12 +672,13 @@ extern "C" int asr_cache4_get(void* stream, const void* codes, const void* meta,
     ASR_REQUIRE(asr_aligned(out, 16) && asr_aligned(codes, 16) && asr_aligned(meta, 4) && strides_ok(st, out_dtype == ASR_F32 ? 4 : 8), ASR_ERR_ALIGN,
                 "cache4_get: rows of out start on 16 bytes, codes on 16, meta on 4");
     hipStream_t hs = static_cast<hipStream_t>(stream);
-    if (out_dtype == ASR_F32)
-        hipLaunchKernelGGL((cache4_get_kernel<float>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<float*>(out), st,
-                           static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta), s);
-    else
-        hipLaunchKernelGGL((cache4_get_kernel<bf16_t>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<bf16_t*>(out), st,
-                           static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta), s);
+    if (out_dtype == ASR_F32) {
+        if (s.rb_log2 == 0) hipLaunchKernelGGL((cache4_get_kernel<float, true>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<float*>(out), st, static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta), s);
+        else hipLaunchKernelGGL((cache4_get_kernel<float, false>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<float*>(out), st, static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta), s);
+    } else {
+        if (s.rb_log2 == 0) hipLaunchKernelGGL((cache4_get_kernel<bf16_t, true>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<bf16_t*>(out), st, static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta), s);
+        else hipLaunchKernelGGL((cache4_get_kernel<bf16_t, false>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<bf16_t*>(out), st, static_cast<const uint32_t*>(codes), static_cast<const uint32_t*>(meta), s);
+    }
     ASR_LAUNCH_CHECK("cache4_get");
     return 0;
 }
@@ -687,7 +707,7 @@ extern "C" int asr_cache4_reorder(void* stream, const void* codes, const void* m
 
 extern "C" int64_t asr_cache4_attention_workspace_bytes(int N, int h, int h_kv, int Lq, int T, int dtype) {
     if (N <= 0 || h_kv <= 0 || h <= 0 || h % h_kv || Lq <= 0 || T <= 0 || (int64_t)N * h_kv > INT32_MAX || (int64_t)(h / h_kv) * Lq > INT32_MAX) return 0;
-    const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T, dtype);
+    const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T);
     return p.splits == 1 ? 0 : (int64_t)N * h * Lq * p.splits * PART * 4;
 }
 
@@ -701,7 +721,7 @@ extern "C" int asr_cache4_attention(void* stream, const void* q, int dtype, int6
     ASR_REQUIRE((int64_t)N * h * Lq <= INT32_MAX / 128, ASR_ERR_UNSUPPORTED, "cache4_attention: more than 2^24 queries");
     ASR_REQUIRE(asr_aligned(q, 4) && asr_aligned(ctx, 4) && asr_aligned(k_codes, 16) && asr_aligned(v_codes, 16) && asr_aligned(k_meta, 4) && asr_aligned(v_meta, 4),
                 ASR_ERR_ALIGN, "cache4_attention: codes start on 16 bytes, the rest on 4");
-    const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T, dtype);
+    const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T);
     const int64_t need = p.splits == 1 ? 0 : (int64_t)N * h * Lq * p.splits * PART * 4;
     ASR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asr_aligned(workspace, 4)), ASR_ERR_ARG, "cache4_attention: workspace of %lld bytes needed, %lld given",
                 (long long)need, (long long)(workspace ? workspace_bytes : 0));
