@@ -410,6 +410,23 @@ class PositionalEncoding(nn.Module):
         return self.pe[0, :length].contiguous()
 
 
+def _attend(q, k, v, k_len, causal, need_lse=False, drop=None, drop_bits=None):
+    """attention over tensors, or over 4-bit caches (decoding: no dropout, no gradient; `causal` is never asked of a cache there)"""
+    if isinstance(k, ops.Cache4):
+        if drop is not None or _TAPE is not None:
+            raise NotImplementedError("a K / V cache in 4 bits serves decoding in eval mode: call model.eval(), or set the decoder's cache_bits / memory_bits to 16")
+        return ops.cache4_attention(q, k, v, k_len, causal, need_lse=need_lse)
+    return ops.attention_fwd(q, k, v, k_len, causal, need_lse=need_lse, drop=drop, drop_bits=drop_bits)
+
+
+def _bits4(module, name):
+    """whether the decoder's `cache_bits` / `memory_bits` asks for 4-bit caches"""
+    bits = getattr(module, name)
+    if bits not in (4, 16):
+        raise ValueError("%s.%s is 16 (the precision's own type) or 4, got %r" % (type(module).__name__, name, bits))
+    return bits == 4
+
+
 class MultiheadAttention(_Cached):
     """src/transformer/attention.py:6-62 (with ScaledDotProductAttention :65-86 fused in)."""
 
@@ -460,7 +477,7 @@ class MultiheadAttention(_Cached):
         else:
             dp_attn = _drop(self, "attention.dropout")   # attention.py:83
             dbits = ops.attention_dropmask(dp_attn, B, h, Lq, Lk, q.device)      # hashed once; forward, dQ and dK/dV kernels read bits
-        ctx, lse = ops.attention_fwd(q, k, v, k_len, causal, need_lse=rec, drop=dp_attn, drop_bits=dbits)
+        ctx, lse = _attend(q, k, v, k_len, causal, need_lse=rec, drop=dp_attn, drop_bits=dbits)
         ctx2, wfc = ctx.view(B * Lq, h * 64), self._w("fc", (self.fc.weight,))
         if _PRECISION == "bf16" and ops.gemm_add_layernorm_ok(ctx2, wfc, xq.f32.shape[1], B, Lq):      # projection + LayerNorm in one launch
             o, y32, y16, mean, rstd = ops.gemm_add_layernorm(ctx2, wfc, self._b("bfc", (self.fc.bias,)), xq.f32, self.layer_norm.weight,
@@ -545,14 +562,20 @@ class MultiheadAttention(_Cached):
         qscale = _LOG2E / math.sqrt(self.d_k)
         if q is None:
             q = ops.proj_heads(xq.mma(), self._w("q", (self.w_qs.weight,)), self._b("bq", (self.w_qs.bias,)), 1, B, Lq, h, qscale)[0]
-        ctx, _ = ops.attention_fwd(q, kv_pre[0], kv_pre[1], k_len, False, need_lse=False, drop=None, drop_bits=None)
+        ctx, _ = _attend(q, kv_pre[0], kv_pre[1], k_len, False, need_lse=False, drop=None, drop_bits=None)
         return ctx.view(B * Lq, h * 64)
 
     def _impl_cached_self(self, x, k_cache, v_cache, t, k_len, next_attn=None, next_lq=1):
         """Self-attention of ONE new position t (x: Act [B*1, d]) against the cache (decoding): its key / value are projected and
         written into k_cache / v_cache [B, h, Tmax, 64] at position t, then the query attends to positions < k_len (= t + 1).
-        bf16, d_model = 256, position on the device: the whole sub-layer is ONE launch (asr_decode_self_attn)."""
+        bf16, d_model = 256, position on the device: the whole sub-layer is ONE launch (asr_decode_self_attn).
+        k_cache an ops.Cache4 stack [K, V] (v_cache None): the caches in 4 bits, one projection, one quantising put, one attention."""
         h, B = self.n_head, x.B
+        if isinstance(k_cache, ops.Cache4):
+            qkv = ops.proj_heads(x.mma(), self._w("qkv", (self.w_qs.weight, self.w_ks.weight, self.w_vs.weight)),
+                                 self._b("bqkv", (self.w_qs.bias, self.w_ks.bias, self.w_vs.bias)), 3, B, 1, h, _LOG2E / math.sqrt(self.d_k))
+            ops.cache4_put(k_cache, qkv[1:], pos=t[:1])
+            return self._impl(x, Act(None, None, B, k_cache.shape[3]), k_len, False, None, kv_pre=(k_cache[0], k_cache[1], None), q_pre=qkv[0])
         # (eval semantics only: the one-launch form has no dropout, like _decode_cross_ffn's; a model left in train() takes the
         # separate launches, whose _drop sites stay active in every sub-layer alike)
         if (_DECODE_FUSED and _PRECISION == "bf16" and not self.training and torch.is_tensor(t) and x.L == 1 and
@@ -1161,8 +1184,23 @@ class _DecodeGraph(dict):
             pass
 
 
+def _step_caches(four_bits, n, N, h, T, cdt, dev):
+    """the self-attention caches of a decoding step, one allocation [K of layer 0, V of layer 0, K of layer 1, ...] -> (what each layer's
+    _impl_cached_self takes, the re-gathering of all of them by parent row)"""
+    if four_bits:
+        cache = ops.Cache4.empty(2 * n, N, h, T, dev)
+        return [(cache[2 * i:2 * i + 2], None) for i in range(n)], lambda parent, state, beam: ops.cache4_reorder(cache, parent, state, beam)
+    cache = torch.zeros((2 * n, N, h, T, 64), device=dev, dtype=cdt)
+    return [(cache[2 * i], cache[2 * i + 1]) for i in range(n)], lambda parent, state, beam: ops.beam_reorder_cache(cache, parent, state, beam)
+
+
 class Decoder(_Cached):
-    """src/transformer/decoder.py:13-96 (forward path; decode loops are out of scope)."""
+    """src/transformer/decoder.py:13-96 (forward path; decode loops are out of scope).
+    `cache_bits` / `memory_bits` (16, or 4; batch_decode and batch_beam_decode): what the self-attention K / V caches and the encoder-side
+    K / V of all layers are held in while a batch is decoded.  16 = the precision's own type (bf16; f32 in the parity mode), 4 = quantised as
+    they are written (ops.Cache4: 4.5 bits a value), a quarter of the bytes every step reads, and hypotheses that may differ."""
+    cache_bits = 16
+    memory_bits = 16
 
     def __init__(self, sos_id, eos_id, n_tgt_vocab, n_layers, n_head, d_model, d_inner, dropout=0.1):
         super().__init__()
@@ -1277,7 +1315,7 @@ class Decoder(_Cached):
         T = int(max_decode_len)
         if T <= 0:
             return torch.zeros((B, 0), dtype=torch.long, device=dev), torch.zeros_like(len_encoded), torch.zeros(0)
-        key = (B, L, T, str(dev), _PRECISION, _PARAM_EPOCH, self.sos_id, self.eos_id, tuple((p.data_ptr(), p._version) for p in self.parameters()))
+        key = (B, L, T, str(dev), _PRECISION, _PARAM_EPOCH, self.cache_bits, self.memory_bits, self.sos_id, self.eos_id, tuple((p.data_ptr(), p._version) for p in self.parameters()))
         dg = self.__dict__.get("_decode_graph")
         if dg is None or dg["key"] != key:
             dg = self._build_decode_graph(B, L, T, dev, key)
@@ -1322,7 +1360,7 @@ class Decoder(_Cached):
             z = torch.zeros((B, beam), dtype=len_encoded.dtype, device=dev)
             return (torch.zeros((B, beam, 0), dtype=torch.long, device=dev), z,
                     torch.tensor([0.0] + [-1e10] * (beam - 1), dtype=torch.float32, device=dev).repeat(B).view(B, beam))
-        key = (B, L, T, beam, str(dev), _PRECISION, _PARAM_EPOCH, self.sos_id, self.eos_id, tuple((p.data_ptr(), p._version) for p in self.parameters()))
+        key = (B, L, T, beam, str(dev), _PRECISION, _PARAM_EPOCH, self.cache_bits, self.memory_bits, self.sos_id, self.eos_id, tuple((p.data_ptr(), p._version) for p in self.parameters()))
         g = self.__dict__.get("_beam_graph")
         if g is None or g["key"] != key:
             self.__dict__["_beam_graph"] = None
@@ -1367,14 +1405,15 @@ class Decoder(_Cached):
         cur = torch.full((N,), self.sos_id, dtype=torch.long, device=dev)
         parent = torch.zeros(N, dtype=torch.long, device=dev)
         n_steps = torch.full((B,), T + 1, dtype=torch.int32, device=dev)          # every utterance takes every step (the <eos> stop is global)
-        cache = torch.zeros((2 * n, N, h, T, 64), device=dev, dtype=cdt)
+        kv, reorder = _step_caches(_bits4(self, "cache_bits"), n, N, h, T, cdt, dev)
+        memory4 = ops.Cache4.empty(2 * n, B, h, L, dev) if _bits4(self, "memory_bits") else None
         emb = self.tgt_word_emb.weight.detach().float()
         pe = self.positional_encoding.pe[0].contiguous()
         box = {}
 
         def prologue():
             enc = Act(enc_buf, None, B, L)
-            box["enc"], box["cross"] = enc, self._cross_kv(enc)
+            box["enc"], box["cross"] = enc, self._cross_kv(enc, memory4, enc_len)
 
         def step():
             with _decode_step():
@@ -1384,18 +1423,18 @@ class Decoder(_Cached):
             x32, x16 = ops.decode_embed(cur, emb, pe, state, want_bf16=(_PRECISION == "bf16"))
             x = Act(x32, x16, N, 1)
             for i, layer in enumerate(self.layer_stack):
-                x = layer.slf_attn._impl_cached_self(x, cache[2 * i], cache[2 * i + 1], state, k_len, next_attn=layer.enc_attn, next_lq=beam)
+                x = layer.slf_attn._impl_cached_self(x, *kv[i], state, k_len, next_attn=layer.enc_attn, next_lq=beam)
                 xq = Act(x.f32, x.b16, B, beam)               # the beams of an utterance: `beam` queries of one cross-attention
                 x = layer._decode_cross_ffn(xq, box["enc"], enc_len, box["cross"](i), N, q=x.next_q)
             # Decoder.step's log-probabilities, log_softmax again (decoder.py:118 + :191), top-k: one launch
             best, ids = ops.lsm_topk_rows(_vocab_proj(self, "prj", self.tgt_word_prj.weight, x), beam, twice=True)
             ops.beam_step(scores, best, ids, preds, state, n_steps, parent, cur, beam)
-            ops.beam_reorder_cache(cache, parent, state, beam)
+            reorder(parent, state, beam)
             ops.beam_advance(state, k_len, cur, self.eos_id, finished, len_decoded)
 
         g = _DecodeGraph(key=key, enc=enc_buf, enc_len=enc_len, state=state, state0=state0, k_len=k_len, finished=finished,
                          len_decoded=len_decoded, preds=preds, scores=scores, scores0=scores0, cur=cur)
-        g.keep = (cache, parent, n_steps, emb, pe, box, prologue, step)     # the captured kernels address these by raw pointer
+        g.keep = (kv, reorder, memory4, parent, n_steps, emb, pe, box, prologue, step)     # the captured kernels address these by raw pointer
         prologue()                      # eager warm-up of both parts: code objects, derived weights, allocator pools
         step()
         torch.cuda.synchronize(dev)
@@ -1428,15 +1467,18 @@ class Decoder(_Cached):
         len_decoded = torch.ones(B, dtype=torch.int64, device=dev)
         preds = torch.zeros((B, T + 1), dtype=torch.long, device=dev)
         cur = torch.zeros(B, dtype=torch.long, device=dev)
-        kc = [torch.zeros((B, h, T, 64), device=dev, dtype=cdt) for _ in range(n)]
-        vc = [torch.zeros((B, h, T, 64), device=dev, dtype=cdt) for _ in range(n)]
+        if _bits4(self, "cache_bits"):
+            kv, _ = _step_caches(True, n, B, h, T, cdt, dev)
+        else:
+            kv = [tuple(torch.zeros((B, h, T, 64), device=dev, dtype=cdt) for _ in range(2)) for _ in range(n)]
+        memory4 = ops.Cache4.empty(2 * n, B, h, L, dev) if _bits4(self, "memory_bits") else None
         emb = self.tgt_word_emb.weight.detach().float()
         pe = self.positional_encoding.pe[0].contiguous()
         box = {}
 
         def prologue():
             enc = Act(enc_buf, None, B, L)
-            box["enc"], box["cross"] = enc, self._cross_kv(enc)
+            box["enc"], box["cross"] = enc, self._cross_kv(enc, memory4, enc_len)
 
         def step():
             with _decode_step():
@@ -1446,7 +1488,7 @@ class Decoder(_Cached):
             x32, x16 = ops.decode_embed(cur, emb, pe, state, want_bf16=(_PRECISION == "bf16"))
             x = Act(x32, x16, B, 1)
             for i, layer in enumerate(self.layer_stack):
-                x = layer.slf_attn._impl_cached_self(x, kc[i], vc[i], state, k_len, next_attn=layer.enc_attn, next_lq=1)
+                x = layer.slf_attn._impl_cached_self(x, *kv[i], state, k_len, next_attn=layer.enc_attn, next_lq=1)
                 x = layer._decode_cross_ffn(x, box["enc"], enc_len, box["cross"](i), B, q=x.next_q)
             ops.argmax_rows(_vocab_proj(self, "prj", self.tgt_word_prj.weight, x), out=cur)      # argmax of log_softmax = argmax of the logits
             ops.decode_advance(cur, preds, state, k_len, finished, len_decoded, self.eos_id)
@@ -1455,7 +1497,7 @@ class Decoder(_Cached):
                          len_decoded=len_decoded, preds=preds, cur=cur)
         # everything the captured kernels address must outlive the capture: the graphs hold raw pointers, not references (the K/V
         # caches live in the ordinary allocator pool - dropped with these closures they would be handed to the next torch.empty)
-        g.keep = (kc, vc, emb, pe, box, prologue, step)
+        g.keep = (kv, memory4, emb, pe, box, prologue, step)
         state.copy_(state0)
         use_graph = os.environ.get("ASR_AMD_DECODE_GRAPH", "1") != "0"
         prologue()                      # eager warm-up of both parts: code objects, derived weights, allocator pools
@@ -1482,16 +1524,20 @@ class Decoder(_Cached):
         att = [layer.enc_attn for layer in self.layer_stack]
         return ([w for a in att for w in (a.w_ks.weight, a.w_vs.weight)], [b for a in att for b in (a.w_ks.bias, a.w_vs.bias)])
 
-    def _cross_kv(self, enc):
+    def _cross_kv(self, enc, memory4=None, enc_len=None):
         """The encoder-side keys / values of every decoder layer depend only on the encoder output: project them with ONE
         [B*L, n_layers*2*h*64] GEMM instead of n_layers narrow ones, and in the backward collect every layer's dK / dV in one
         [B*L, n_layers*2*h*64] buffer so the weight gradient and the gradient wrt the encoder output are one GEMM each (K = 3072
-        instead of six K = 512 passes that each re-read and re-write the [B*L, d_model] accumulator)."""
+        instead of six K = 512 passes that each re-read and re-write the [B*L, d_model] accumulator).
+        memory4 (decoding): an ops.Cache4 of 2 * n_layers caches the projected rows are quantised into, frames < enc_len only."""
         ws, bs = self.cross_kv_params()
         n, h = len(self.layer_stack), self.n_head
         hd = h * 64
         W, bias = self._w("cross_kv", tuple(ws)), self._b("cross_kvb", tuple(bs))
         kv = ops.proj_heads(enc.mma(), W, bias, 2 * n, enc.B, enc.L, h, 1.0)
+        if memory4 is not None:
+            ops.cache4_put(memory4, kv, n_new=enc_len)
+            kv = memory4
         if _TAPE is None:
             return lambda i: (kv[2 * i], kv[2 * i + 1], None)
         box = {}
@@ -1520,7 +1566,8 @@ class Decoder(_Cached):
 
 
 class Decoder_CIF(_Cached):
-    """src/transformer/decoder.py:327-399 (forward path)."""
+    """src/transformer/decoder.py:327-399 (forward path).  `cache_bits` (16, or 4): as Decoder's, for batch_recognize_beam."""
+    cache_bits = 16
 
     def __init__(self, sos_id, n_tgt_vocab, n_layers, n_head, d_model, d_inner, dropout=0.1):
         super().__init__()
@@ -1658,7 +1705,7 @@ class Decoder_CIF(_Cached):
             raise ValueError("recognize_beam: %d steps asked of %d integrated frames" % (steps, Umax))
         if steps > 0:
             Tmax = max(32, (steps + 31) // 32 * 32)
-            key = (B, beam, Tmax, D, str(dev), _PRECISION, _PARAM_EPOCH, self.sos_id, tuple((p.data_ptr(), p._version) for p in self.parameters()))
+            key = (B, beam, Tmax, D, str(dev), _PRECISION, _PARAM_EPOCH, self.cache_bits, self.sos_id, tuple((p.data_ptr(), p._version) for p in self.parameters()))
             g = self.__dict__.get("_beam_graph")
             if g is None or g["key"] != key:
                 self.__dict__["_beam_graph"] = None
@@ -1690,7 +1737,7 @@ class Decoder_CIF(_Cached):
         state0 = torch.tensor([0, -1], dtype=torch.int32, device=dev)
         state = state0.clone()
         k_len = torch.ones(N, dtype=torch.int32, device=dev)
-        cache = torch.zeros((2 * n, N, h, Tmax, 64), device=dev, dtype=cdt)        # [K of layer 0, V of layer 0, K of layer 1, ...]
+        kv, reorder = _step_caches(_bits4(self, "cache_bits"), n, N, h, Tmax, cdt, dev)
         preds = torch.full((N, Tmax + 1), self.sos_id, dtype=torch.long, device=dev)
         scores0 = torch.tensor([0.0] + [-1e10] * (beam - 1), dtype=torch.float32, device=dev).repeat(B)
         scores = scores0.clone()
@@ -1707,17 +1754,17 @@ class Decoder_CIF(_Cached):
             cat1 = ops.beam_cat_frames(frames, state, beam, cur=cur, emb=emb, pe=pe)            # decoder.py:407-408
             x = Act(ops.gemm_nt(cat1, self._w("inaff", (self.input_affine.weight,)), None), None, N, 1)
             for j, layer in enumerate(self.layer_stack):
-                x = layer.slf_attn._impl_cached_self(x, cache[2 * j], cache[2 * j + 1], state, k_len)
+                x = layer.slf_attn._impl_cached_self(x, *kv[j], state, k_len)
                 x = layer.pos_ffn._impl(x, None)
             cat2 = Act(ops.beam_cat_frames(frames, state, beam, other=x.f32.contiguous()), None, N, 1)     # decoder.py:416
             best, ids = ops.lsm_topk_rows(_vocab_proj(self, "prj", self.tgt_word_prj.weight, cat2), beam)
             ops.beam_step(scores, best, ids, preds, state, n_steps, parent, cur, beam)
-            ops.beam_reorder_cache(cache, parent, state, beam)
+            reorder(parent, state, beam)
             ops.beam_advance(state, k_len)
 
         g = _DecodeGraph(key=key, frames=frames, n_steps=n_steps, state=state, state0=state0, k_len=k_len, preds=preds, scores=scores,
                          scores0=scores0, cur=cur)
-        g.keep = (cache, parent, emb, pe, step)     # the captured kernels address these by raw pointer
+        g.keep = (kv, reorder, parent, emb, pe, step)     # the captured kernels address these by raw pointer
         n_steps.fill_(1)
         step()                          # eager warm-up: code objects, derived weights, allocator pools
         torch.cuda.synchronize(dev)

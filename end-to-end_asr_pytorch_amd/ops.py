@@ -1384,7 +1384,7 @@ def beam_advance(state, k_len, cur=None, eos_id=0, finished=None, len_decoded=No
 # ask a tensor for each property once - 6-7 us a call on the host instead of 13.)
 class Cache4:
     """A K / V cache in 4 bits (asr_hip.h: asr_cache4_put): `codes` uint8 [n_kv, N, h, Tmax, 32] and `meta` bf16 [n_kv, N, h, Tmax, 2] - or both
-    without the first dimension, one cache (`cache[i]` of a stack: views of the same memory).  4.5 bits a value against 16 or 32.
+    without the first dimension, one cache (`cache[i]` of a stack, or a stack `cache[i:j]`: views of the same memory).  4.5 bits a value against 16 or 32.
     `shape` = (n_kv, N, h, Tmax), n_kv = 1 for one cache."""
     __slots__ = ("codes", "meta", "shape", "stack", "device")
 
