@@ -1380,8 +1380,8 @@ def beam_advance(state, k_len, cur=None, eos_id=0, finished=None, len_decoded=No
 
 
 # ---- K / V cache held in 4 bits (csrc/cache4.hip) -------------------------------------------------------------------------------
-# (A token's calls are a few microseconds of GPU work each and a step makes dozens of them: these wrappers pass plain integers to ctypes and
-# ask a tensor for each property once - 6-7 us a call on the host instead of 13.)
+# (A token's calls are a few microseconds of GPU work each: the wrappers pass plain integers to ctypes and ask a tensor for each property
+# once.  Of 6-7 us on the host, 2.7 are the launch, 1 ctypes and 1.4 the output's allocation.)
 class Cache4:
     """A K / V cache in 4 bits (asr_hip.h: asr_cache4_put): `codes` uint8 [n_kv, N, h, Tmax, 32] and `meta` bf16 [n_kv, N, h, Tmax, 2] - or both
     without the first dimension, one cache (`cache[i]` of a stack, or a stack `cache[i:j]`: views of the same memory).  4.5 bits a value against 16 or 32.
@@ -1391,16 +1391,17 @@ class Cache4:
     def __init__(self, codes, meta):
         if codes.dtype is not torch.uint8 or meta.dtype is not torch.bfloat16:
             raise TypeError("Cache4: codes are uint8 and meta bfloat16, got %s and %s" % (codes.dtype, meta.dtype))
-        cs, ms = tuple(codes.shape), tuple(meta.shape)
-        if len(cs) not in (4, 5) or cs[-1] != 32 or ms[-1] != 2 or cs[:-1] != ms[:-1]:
-            raise ValueError("Cache4: codes [.., N, h, Tmax, 32] and meta [.., N, h, Tmax, 2], got %s and %s" % (cs, ms))
+        *lead, nb = codes.shape
+        *same, nm = meta.shape
+        if len(lead) not in (3, 4) or nb != 32 or nm != 2 or lead != same:
+            raise ValueError("Cache4: codes [.., N, h, Tmax, 32] and meta [.., N, h, Tmax, 2], got %s and %s" % (tuple(codes.shape), tuple(meta.shape)))
         if not (codes.is_contiguous() and meta.is_contiguous()):
             raise ValueError("Cache4: codes and meta are contiguous")
         self.device = codes.get_device()
         if self.device != meta.get_device():
             raise ValueError("Cache4: codes on %s, meta on %s" % (codes.device, meta.device))
-        self.codes, self.meta, self.stack = codes, meta, len(cs) == 5
-        self.shape = cs[:-1] if len(cs) == 5 else (1,) + cs[:-1]
+        self.codes, self.meta, self.stack = codes, meta, len(lead) == 4
+        self.shape = tuple(lead) if self.stack else (1, *lead)
 
     @classmethod
     def empty(cls, n_kv, N, h, Tmax, device):
@@ -1428,7 +1429,7 @@ def _cache4_call(what, fn, cache, ts, args):
     if dev != torch._C._cuda_getDevice():
         with torch.cuda.device(dev):
             return check(fn(_stream(), *args), what)
-    rc = fn(_stream(), *args)
+    rc = fn(_raw_stream(dev) if _raw_stream is not None else _stream(), *args)
     if rc:
         check(rc, what)
 
@@ -1451,12 +1452,12 @@ def _cache4_slots(what, N, pos, n_tok):
 
 def _cache4_strides(what, t):
     """element strides of rows of 64 adjacent values; a dimension of one element has none"""
-    st = t.stride()
-    if t.is_contiguous():
-        return st[:-1] if 1 not in t.shape else [v if v % 64 == 0 else 0 for v in st[:-1]]      # (a size-1 dimension's stride is arbitrary)
-    if st[-1] != 1:
+    *st, last = t.stride()
+    if last != 1:
         raise ValueError("%s: the 64 values of a row are adjacent" % what)
-    return [0 if n == 1 else v for n, v in zip(t.shape[:-1], st)]
+    if 1 in t.shape:      # (whose stride is arbitrary)
+        st = [0 if n == 1 else v for n, v in zip(t.shape, st)]
+    return st
 
 
 def cache4_put(cache, x, pos=None, n_new=None):
@@ -1501,10 +1502,9 @@ def cache4_attention(q, k_cache, v_cache, k_len=None, causal=False, need_lse=Fal
     """attention_fwd over 4-bit caches of N rows (one K, one V: `cache[2 * i]`, `cache[2 * i + 1]`): q [N, h, Lq, 64] (pre-scaled, any strides with
     adjacent rows of 64), h a multiple of the caches' heads -> ctx [N, Lq, h*64] in q's dtype, lse f32 [N, h, Lq] or None.  k_len int32 [N] or
     None; causal: the Lq queries are the last tokens of each row.  A query that sees nothing gets zeros (lse -inf)."""
-    qs = tuple(q.shape)
-    if len(qs) != 4 or qs[3] != 64:
-        raise ValueError("cache4_attention: q is [N, h, Lq, 64], got %s" % (qs,))
-    N, h, Lq, _ = qs
+    if q.dim() != 4 or q.shape[3] != 64:
+        raise ValueError("cache4_attention: q is [N, h, Lq, 64], got %s" % (tuple(q.shape),))
+    N, h, Lq, _ = q.shape
     _, n, h_kv, T = k_cache.shape
     if k_cache.stack or v_cache.stack or v_cache.shape != k_cache.shape or n != N or h_kv == 0 or h % h_kv:
         raise ValueError("cache4_attention: caches [N, h_kv, T] with N = %d and h_kv dividing %d, got %s and %s" %
@@ -1512,7 +1512,7 @@ def cache4_attention(q, k_cache, v_cache, k_len=None, causal=False, need_lse=Fal
     if k_len is not None and (k_len.dtype is not torch.int32 or k_len.numel() != N or not k_len.is_contiguous()):
         raise ValueError("cache4_attention: k_len is a contiguous int32 tensor of %d elements" % N)
     code = dtype_code(q)
-    st = _cache4_strides("cache4_attention", q)
+    st = (h * Lq * 64, Lq * 64, 64) if q.is_contiguous() else _cache4_strides("cache4_attention", q)
     ctx = q.new_empty((N, Lq, h * 64))
     lse = q.new_empty((N, h, Lq), dtype=torch.float32) if need_lse else None
     if N * h * Lq:
