@@ -151,7 +151,7 @@ SIGNATURES = {
     "asr_cache4_put": [_vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i],
     "asr_cache4_get": [_vp, _vp, _vp, _vp, _i, _i64, _i64, _i64, _i64, _vp, _i, _vp, _i, _i, _i, _i, _i],
     "asr_cache4_reorder": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i],
-    "asr_cache4_attention_workspace_bytes": [_i, _i, _i, _i, _i, _i],
+    "asr_cache4_attention_workspace_bytes": [_i, _i, _i, _i, _i],
     "asr_cache4_attention": [_vp, _vp, _i, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i, _vp, _i64],
     "asr_add2d": [_vp, _vp, _i64, _vp, _i64, _i, _i],
     "asr_add_transposed": [_vp, _vp, _vp, _i, _i, _i, _i64],

@@ -59,6 +59,10 @@ __device__ __forceinline__ float quotient(float d, float s, float rs) {
     return __builtin_fmaf(__builtin_fmaf(-y, s, d), rs, y);
 }
 
+// Quantising reads 128 (bf16) or 256 bytes a row and writes 36: HBM, with the VALU next to it (11 instructions a value).  4 lanes a row share the
+// row's own arithmetic (8 lanes: 3 instructions a value more); the next row's loads are in flight while this one is worked on.  Measured:
+// 12 x 32 x 4 rows of 1000 tokens in bf16 53 us = 4.7 TB/s (a copy of 1 GiB moves 5.2 here); 47 us = 4.0 with rows of 500 to 1000 tokens.
+//
 // The codes of 16 values of a row whose 64 values lie in 4 neighbouring lanes: -> the two 32-bit words of nibbles, and the row's (scale, mid).
 // Every decision is that of (x - mid) / scale computed exactly.  The corrected quotient settles it unless the subtraction was rounded and
 // the quotient is next to a border:
@@ -175,6 +179,8 @@ __global__ __launch_bounds__(256) void cache4_put_kernel(const T* __restrict__ x
     }
 }
 
+// Reading back: 36 bytes in, 128 or 256 out.  8 lanes a row, 16 bytes (bf16) of output each: whole cache lines per store.  Measured: 12 x 32 x 4
+// rows of 1000 tokens to bf16 44 us = 5.7 TB/s.
 template <typename T, bool ONE_ROW>
 __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, strides_t st, const uint32_t* __restrict__ codes,
                                                          const uint32_t* __restrict__ meta, slots_t s) {
@@ -200,7 +206,8 @@ __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, st
 // ---- re-gathering by parent ------------------------------------------------------------------------------------------------------------
 // A group is one (kv, utterance, head).  A block takes 256 pieces of its positions - 16-byte halves of the codes, or meta words - and a thread
 // its piece for all the beam's rows: it reads every source row's before it writes any, so source and destination may be the same cache.  The
-// parents are the same for a whole block: scalar loads, row addresses in scalar registers.
+// parents are the same for a whole block: scalar loads, row addresses in scalar registers (with them in vector registers: 236 VGPRs, 70 us).
+// Measured: 12 x 8 utterances x 8 beams x 4 heads x 777 positions into another cache 38.5 us = 4.5 TB/s; a step of 32 x 5 beams, 51 positions 7 us.
 template <typename V, int BEAM> __device__ __forceinline__ void regather(const V* src, V* dst, const int64_t* parent, int64_t first, int64_t row, int beam, unsigned u,
                                                                          bool in_place) {
     V v[BEAM];
@@ -252,6 +259,10 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
 // The running reference m of a query is renewed only when a score passes it by 2^32 (weights are f32 and scaled per tile: nothing needs
 // them below 1), so a tile costs one reduction across the wave per query, the largest weight's, and four queries share its steps.
 // The next tile's loads are issued before the present one is worked on, the first tile's before the query is.
+//
+// What bounds it: HBM for long rows (72 bytes a token and head; 4 rows x 4 heads of 100003 slots, 16 splits: 19.5 us = 4.4 TB/s, + 3.9 us for
+// the join), launch and one chain of loads for a decoding step (32 x 4 rows of 1000 slots: 5.3 us with one query, 7.0 with five), the VALU
+// for chunks (33 queries x 64 rows of up to 2011 slots: 14.7 us; about 110 instructions a tile and 18 a tile and query).
 template <int ND> struct Digits {
     static constexpr float UNIT = ND == 2 ? 127.f * 256.f : 127.f * 65536.f;      // the integer that the largest element becomes
     static constexpr int BIAS = ND == 2 ? 0x80 : 0x8080;                          // u + BIAS, its lower bytes' sign bits inverted: the digits, lowest first
@@ -583,7 +594,14 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void cache4_join_kernel(attn4_t a)
     if (a.lse && lane == 0) a.lse[((int64_t)n * a.h + head) * a.Lq + i] = L == 0.f ? -INFINITY : M + __log2f(L);
 }
 
-// How a call is cut: queries per block, splits of the keys.
+// How a call is cut.  Times in us, bf16, graph replays, keys cold where they do not fit the caches.
+//   queries a block   up to 4, evenly: eight need 184 VGPRs instead of 106 and lose at every size (5 queries x 128 rows x 1000 slots 8.4 against
+//                     7.1, 33 queries x 64 rows x 2011 slots 17.0 against 14.7)
+//   waves             one per tile of 64 slots up to 8; 4 where there are two blocks a CU and more anyway (640 rows x 1000 slots 12.1 with 8,
+//                     11.7 with 4; 128 rows 5.8 with 8, 5.9 with 4, 7.7 with 2)
+//   splits            where a wave would walk more than 4 tiles and there are no more than 128 blocks: as many as fill 256 CUs with a block each,
+//                     two tiles a wave at least (16 rows x 100003 slots: 1 split 168, 16 splits 26.6, 32 splits 27.8; 4 rows: 32 splits 11.6, 20
+//                     13.4).  Below that the second launch costs more than it gives (20 rows x 777 slots 4.9 against 6.4).
 struct plan_t { int nq, qtiles, splits, waves; };
 plan_t attn_plan(int rows, int Q, int T) {
     plan_t p;
@@ -705,7 +723,7 @@ extern "C" int asr_cache4_reorder(void* stream, const void* codes, const void* m
     return 0;
 }
 
-extern "C" int64_t asr_cache4_attention_workspace_bytes(int N, int h, int h_kv, int Lq, int T, int dtype) {
+extern "C" int64_t asr_cache4_attention_workspace_bytes(int N, int h, int h_kv, int Lq, int T) {
     if (N <= 0 || h_kv <= 0 || h <= 0 || h % h_kv || Lq <= 0 || T <= 0 || (int64_t)N * h_kv > INT32_MAX || (int64_t)(h / h_kv) * Lq > INT32_MAX) return 0;
     const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T);
     return p.splits == 1 ? 0 : (int64_t)N * h * Lq * p.splits * PART * 4;
@@ -719,8 +737,8 @@ extern "C" int asr_cache4_attention(void* stream, const void* q, int dtype, int6
     ASR_REQUIRE(N > 0 && h > 0 && h_kv > 0 && Lq > 0 && T > 0 && h % h_kv == 0, ASR_ERR_ARG, "cache4_attention: bad sizes (N=%d h=%d h_kv=%d Lq=%d T=%d)", N, h, h_kv, Lq, T);
     ASR_REQUIRE(T <= CACHE4_MAX_T, ASR_ERR_UNSUPPORTED, "cache4_attention: more than 2^24 slots");
     ASR_REQUIRE((int64_t)N * h * Lq <= INT32_MAX / 128, ASR_ERR_UNSUPPORTED, "cache4_attention: more than 2^24 queries");
-    ASR_REQUIRE(asr_aligned(q, 4) && asr_aligned(ctx, 4) && asr_aligned(k_codes, 16) && asr_aligned(v_codes, 16) && asr_aligned(k_meta, 4) && asr_aligned(v_meta, 4),
-                ASR_ERR_ALIGN, "cache4_attention: codes start on 16 bytes, the rest on 4");
+    ASR_REQUIRE(asr_aligned(q, dtype == ASR_F32 ? 4 : 2) && asr_aligned(ctx, dtype == ASR_F32 ? 4 : 2) && asr_aligned(k_codes, 16) && asr_aligned(v_codes, 16) && asr_aligned(k_meta, 4) && asr_aligned(v_meta, 4),
+                ASR_ERR_ALIGN, "cache4_attention: codes start on 16 bytes, meta on 4, q and ctx on their elements");
     const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T);
     const int64_t need = p.splits == 1 ? 0 : (int64_t)N * h * Lq * p.splits * PART * 4;
     ASR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asr_aligned(workspace, 4)), ASR_ERR_ARG, "cache4_attention: workspace of %lld bytes needed, %lld given",

@@ -1469,7 +1469,7 @@ def cache4_put(cache, x, pos=None, n_new=None):
         raise ValueError("cache4_put: x is [.., L, 64] with the cache's leading dimensions %s, got %s" % (tuple(cache.codes.shape[:-2]), xs))
     st = _cache4_strides("cache4_put", x)
     ps = _cache4_slots("cache4_put", N, pos, n_new)
-    if x.numel() == 0:
+    if x.numel() == 0 or Tmax == 0:
         return
     _cache4_call("asr_cache4_put", lib().asr_cache4_put, cache, (x, pos, n_new),
                  (x.data_ptr(), dtype_code(x), st[0] if cache.stack else 0, *st[-3:], cache.codes.data_ptr(), cache.meta.data_ptr(), _ptr(pos), ps, _ptr(n_new), n_kv, N,
@@ -1486,6 +1486,8 @@ def cache4_get(cache, L=None, pos=None, n_tok=None, dtype=torch.bfloat16):
     ps = _cache4_slots("cache4_get", N, pos, n_tok)
     out = cache.meta.new_empty((n_kv, N, h, L, 64) if cache.stack else (N, h, L, 64), dtype=dtype)
     code = dtype_code(out)
+    if Tmax == 0:
+        return out.zero_()
     if out.numel():
         _cache4_call("asr_cache4_get", lib().asr_cache4_get, cache, (pos, n_tok),
                      (cache.codes.data_ptr(), cache.meta.data_ptr(), out.data_ptr(), code, N * h * L * 64, h * L * 64, L * 64, 64, _ptr(pos), ps, _ptr(n_tok), n_kv, N, h,
@@ -1494,8 +1496,8 @@ def cache4_get(cache, L=None, pos=None, n_tok=None, dtype=torch.bfloat16):
 
 
 @functools.lru_cache(maxsize=1024)
-def _cache4_workspace(N, h, h_kv, Lq, T, code):
-    return lib().asr_cache4_attention_workspace_bytes(N, h, h_kv, Lq, T, code)      # (a function of the sizes alone)
+def _cache4_workspace(N, h, h_kv, Lq, T):
+    return lib().asr_cache4_attention_workspace_bytes(N, h, h_kv, Lq, T)      # (a function of the sizes alone)
 
 
 def cache4_attention(q, k_cache, v_cache, k_len=None, causal=False, need_lse=False):
@@ -1515,8 +1517,10 @@ def cache4_attention(q, k_cache, v_cache, k_len=None, causal=False, need_lse=Fal
     st = (h * Lq * 64, Lq * 64, 64) if q.is_contiguous() else _cache4_strides("cache4_attention", q)
     ctx = q.new_empty((N, Lq, h * 64))
     lse = q.new_empty((N, h, Lq), dtype=torch.float32) if need_lse else None
+    if T == 0:      # (a cache without slots: nothing to see)
+        return ctx.zero_(), lse if lse is None else lse.fill_(float("-inf"))
     if N * h * Lq:
-        nbytes = _cache4_workspace(N, h, h_kv, Lq, T, code)
+        nbytes = _cache4_workspace(N, h, h_kv, Lq, T)
         ws = q.new_empty((nbytes,), dtype=torch.uint8) if nbytes else None
         args = (q.data_ptr(), code, *st, k_cache.codes.data_ptr(), k_cache.meta.data_ptr(), v_cache.codes.data_ptr(), v_cache.meta.data_ptr(), ctx.data_ptr(), _ptr(lse),
                 N, h, h_kv, Lq, T, _ptr(k_len), 1 if causal else 0, _ptr(ws), nbytes)

@@ -655,7 +655,7 @@ int asr_beam_advance(void* stream, int32_t* state, int32_t* k_len, int N, const 
  *   slots that no token goes to are left as they were.
  * asr_cache4_get:  the inverse: out[.., i, :] = the values of slot pos[..] + i for i < n_tok[n], zeros behind (and for slots outside the cache).
  * asr_cache4_reorder:  the rows of utterance b, b * beam .. b * beam + beam - 1 of the N = B * beam rows, re-gathered by `parent` (int64
- *   [N], global row ids) for positions <= state[0], like asr_beam_reorder_cache; out_codes / out_meta = codes / meta: in place; another cache:
+ *   [N], global row ids) for positions <= state[0], like asr_beam_reorder_cache (an id outside its utterance is cut to it); out_codes / out_meta = codes / meta: in place; another cache:
  *   its positions > state[0] are left as they were.  beam <= 8.
  * asr_cache4_attention:  asr_attention_fwd over one K and one V cache of N rows: q (f32 | bf16) [N, h, Lq, 64] by element strides, PRE-MULTIPLIED by
  *   log2(e)/sqrt(64) as there; h a multiple of h_kv, query head i reads key head i / (h / h_kv); ctx [N, Lq, h * 64] in q's dtype; lse f32
@@ -669,7 +669,7 @@ int asr_cache4_get(void* stream, const void* codes, const void* meta, void* out,
                    int64_t s_tok, const int32_t* pos, int pos_stride, const int32_t* n_tok, int n_kv, int N, int h, int L, int Tmax);
 int asr_cache4_reorder(void* stream, const void* codes, const void* meta, void* out_codes, void* out_meta, const int64_t* parent,
                        const int32_t* state, int n_kv, int B, int beam, int h, int Tmax);
-int64_t asr_cache4_attention_workspace_bytes(int N, int h, int h_kv, int Lq, int T, int dtype);
+int64_t asr_cache4_attention_workspace_bytes(int N, int h, int h_kv, int Lq, int T);
 int asr_cache4_attention(void* stream, const void* q, int dtype, int64_t s_n, int64_t s_head, int64_t s_tok, const void* k_codes,
                          const void* k_meta, const void* v_codes, const void* v_meta, void* ctx, float* lse, int N, int h, int h_kv, int Lq, int T,
                          const int32_t* k_len, int causal, void* workspace, int64_t workspace_bytes);

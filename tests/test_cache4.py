@@ -20,6 +20,7 @@ def test_cache4_shapes_and_views():
     assert ops.Cache4.empty(None, 3, 4, 8, "cpu").shape == (1, 3, 4, 8)
     with pytest.raises(IndexError):
         c[0][0]
+    assert c[2:4].shape == (2, 3, 4, 8) and c[2:4].codes.data_ptr() == c[2].codes.data_ptr()
 
 
 @pytest.mark.parametrize("codes,meta,err", [
@@ -105,11 +106,11 @@ def test_library_refuses_before_it_launches():
         return L.asr_cache4_attention(None, p(q) if q else None, dt, 0, 0, 0, p(kc), p(), p(), p(), p(), None, *sizes, None, 0, p(ws) if ws else None, wsb)
     assert attn(q=0) == -1 and attn(dt=2) == -1 and attn(sizes=(1, 4, 3, 1, 8)) == -1 and attn(sizes=(1, 4, 4, 0, 8)) == -1 and attn(kc=72) == -2
     assert attn(sizes=(1, 4, 4, 1, (1 << 24) + 1)) == -3 and attn(sizes=(1 << 12, 1 << 10, 1, 64, 8)) == -3
-    need = L.asr_cache4_attention_workspace_bytes(1, 4, 4, 1, 100000, 1)
+    need = L.asr_cache4_attention_workspace_bytes(1, 4, 4, 1, 100000)
     assert need > 0 and need % 4 == 0
     assert attn(sizes=(1, 4, 4, 1, 100000)) == -1 and b"workspace" in L.asr_last_error()
     assert attn(sizes=(1, 4, 4, 1, 100000), ws=64, wsb=need - 4) == -1
-    assert L.asr_cache4_attention_workspace_bytes(1, 4, 4, 1, 8, 1) == 0 and L.asr_cache4_attention_workspace_bytes(1, 4, 3, 1, 8, 1) == 0
+    assert L.asr_cache4_attention_workspace_bytes(1, 4, 4, 1, 8) == 0 and L.asr_cache4_attention_workspace_bytes(1, 4, 3, 1, 8) == 0
 
 
 def test_header_revision():

@@ -197,6 +197,11 @@ def test_empty_calls():
     assert ops.cache4_get(c, L=0).shape == (2, 3, 4, 0, 64)
     ctx, lse = ops.cache4_attention(torch.zeros(3, 4, 0, 64, device=DEV), c[0], c[1], need_lse=True)
     assert ctx.shape == (3, 0, 256) and lse.shape == (3, 4, 0)
+    bare = ops.Cache4.empty(2, 3, 4, 0, DEV)                                 # no slots
+    ops.cache4_put(bare, torch.ones(2, 3, 4, 2, 64, device=DEV))
+    assert int(ops.cache4_get(bare, L=2).abs().sum()) == 0
+    ctx, lse = ops.cache4_attention(torch.ones(3, 4, 2, 64, device=DEV), bare[0], bare[1], need_lse=True)
+    assert int(ctx.abs().sum()) == 0 and bool(torch.isinf(lse).all())
     none = ops.Cache4.empty(2, 0, 4, 8, DEV)
     assert ops.cache4_attention(torch.zeros(0, 4, 1, 64, device=DEV), none[0], none[1])[0].shape == (0, 1, 256)
 
