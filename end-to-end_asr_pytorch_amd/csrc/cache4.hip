@@ -296,7 +296,7 @@ struct MaxPos {      // non-negative floats as their bit patterns (a NaN stays t
 };
 struct MaxF {
     static __device__ __forceinline__ uint32_t f(uint32_t a, uint32_t b) {
-        return __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+        return __builtin_bit_cast(uint32_t, __builtin_elementwise_maximum(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));      // (a NaN stays)
     }
 };
 struct SumF {
@@ -462,17 +462,16 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
             top = fmaxf(top, e[q]);
         }
         if (__builtin_amdgcn_ballot_w64(top > 32.f)) {
-            float al[NQ];
-#pragma unroll
-            for (int q = 0; q < NQ; ++q) {
-                const float mn = fmaxf(m[q], wave_all<MaxF>(s[q]) * unit[q]);
-                al[q] = __builtin_amdgcn_exp2f(m[q] - mn);
-                m[q] = mn; l[q] *= al[q]; mv[q] *= al[q];
-                e[q] = __builtin_fmaf(s[q], unit[q], -mn);
-            }
+            const float big = NQ == 1 ? wave_all<MaxF>(s[0]) : wave_four<MaxF>(s[0], s[NQ > 1 ? 1 : 0], s[NQ > 2 ? 2 : 0], s[NQ > 3 ? 3 : 0]);      // of query c
             float f = 1.f;
 #pragma unroll
-            for (int q = 0; q < NQ; ++q) f = c == q ? al[q] : f;
+            for (int q = 0; q < NQ; ++q) {
+                const float mn = __builtin_elementwise_maximum(m[q], __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, big), 16 * q)) * unit[q]);
+                const float al = __builtin_amdgcn_exp2f(m[q] - mn);
+                m[q] = mn; l[q] *= al; mv[q] *= al;
+                e[q] = __builtin_fmaf(s[q], unit[q], -mn);
+                f = c == q ? al : f;
+            }
 #pragma unroll
             for (int d = 0; d < 4; ++d) acc[d] *= f;
         }
