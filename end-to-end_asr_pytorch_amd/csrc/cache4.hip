@@ -490,6 +490,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
             w[q] = p * (seen ? vsc : 0.f);
         }
         const float most = NQ == 1 ? wave_all<MaxPos>(w[0]) : wave_four<MaxPos>(w[0], w[1], w[2], w[3]);      // of query c
+        // (UNIT / most has to be finite: weights below 1e-30 of a reference that is within 2^32 of the largest probability count as 0)
         const float inv = most > 1e-30f ? D::UNIT * __builtin_amdgcn_rcpf(most) : 0.f, wunit = most * (1.f / (16.f * D::UNIT));
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
@@ -596,8 +597,8 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void cache4_join_kernel(attn4_t a)
 // How a call is cut.  Times in us, bf16, graph replays, keys cold where they do not fit the caches.
 //   queries a block   up to 4, evenly: eight need 184 VGPRs instead of 106 and lose at every size (5 queries x 128 rows x 1000 slots 8.4 against
 //                     7.1, 33 queries x 64 rows x 2011 slots 17.0 against 14.7)
-//   waves             one per tile of 64 slots up to 8; 4 where there are two blocks a CU and more anyway (640 rows x 1000 slots 12.1 with 8,
-//                     11.7 with 4; 128 rows 5.8 with 8, 5.9 with 4, 7.7 with 2)
+//   waves             one per tile of 64 slots up to 8; 4 where more blocks than CUs make a CU take two anyway (300 rows x 2000 slots 12.6 with 8,
+//                     11.6 with 4; 230 rows 8.8 and 9.3; 128 rows x 1000 slots 5.8 with 8, 5.9 with 4, 7.7 with 2)
 //   splits            where a wave would walk more than 4 tiles and there are no more than 128 blocks: as many as fill 256 CUs with a block each,
 //                     two tiles a wave at least (16 rows x 100003 slots: 1 split 168, 16 splits 26.6, 32 splits 27.8; 4 rows: 32 splits 11.6, 20
 //                     13.4).  Below that the second launch costs more than it gives (20 rows x 777 slots 4.9 against 6.4).
@@ -608,7 +609,7 @@ plan_t attn_plan(int rows, int Q, int T) {
     p.nq = (Q + p.qtiles - 1) / p.qtiles;
     const int tiles = (T + 63) / 64;
     const int64_t blocks = (int64_t)rows * p.qtiles;
-    const int most = blocks >= 512 ? 4 : 8;
+    const int most = blocks > 256 ? 4 : 8;
     p.waves = 1;
     while (p.waves < most && p.waves < tiles) p.waves *= 2;
     p.splits = 1;

@@ -643,7 +643,7 @@ int asr_beam_advance(void* stream, int32_t* state, int32_t* k_len, int N, const 
  * A cache of n_kv x N x h rows of Tmax slots (kv = K of layer 0, V of layer 0, K of layer 1, ...; h = key heads): a slot is the 64 values of
  * one head of one token.
  *   codes  uint8 [n_kv, N, h, Tmax, 32]   signed 4-bit codes: byte j holds value 2j in its low nibble and value 2j + 1 in its high one
- *   meta   bf16  [n_kv, N, h, Tmax, 2]    (scale, mid);  the value a code stands for is mid + scale * code
+ *   meta   bf16  [n_kv, N, h, Tmax, 2]    (scale >= 0, mid);  the value a code stands for is mid + scale * code
  * Both contiguous; codes start on 16 bytes, meta on 4.  4.5 bits a value.  Quantising (asr_cache4_put), per slot:
  *   span = max - min (f32);  scale = bf16(span / 15), 0 where span < 2^-100;  mid = bf16(min + 8 * scale)
  *   code = (x - mid) / scale rounded to the nearest integer, ties to even - decided exactly, not from a rounded quotient -, cut to [-8, 7]
@@ -661,7 +661,8 @@ int asr_beam_advance(void* stream, int32_t* state, int32_t* k_len, int N, const 
  *   log2(e)/sqrt(64) as there; h a multiple of h_kv, query head i reads key head i / (h / h_kv); ctx [N, Lq, h * 64] in q's dtype; lse f32
  *   [N, h, Lq] (base 2) or NULL.  Slot j of row n is visible iff j < k_len[n] (int32 [N], cut to [0, T]; NULL: T) and, with `causal`, j <=
  *   k_len[n] - Lq + i for query i: the Lq queries are the last tokens of the row.  A query that sees nothing gets zeros and lse = -inf.
- *   Masked slots may hold anything.  workspace: asr_cache4_attention_workspace_bytes() bytes (0: none needed), contents irrelevant, not shared
+ *   Masked slots may hold anything.  Queries whose largest element is under 2^-100, and value scales times probability under 1e-30, count as
+ *   0.  workspace: asr_cache4_attention_workspace_bytes() bytes (0: none needed), contents irrelevant, not shared
  *   by two launches that may run concurrently. */
 int asr_cache4_put(void* stream, const void* x, int x_dtype, int64_t s_kv, int64_t s_n, int64_t s_head, int64_t s_tok, void* codes, void* meta,
                    const int32_t* pos, int pos_stride, const int32_t* n_new, int n_kv, int N, int h, int L, int Tmax);
