@@ -91,7 +91,18 @@ def test_cif_decoder_in_4_bits(monkeypatch):
 
 @pytest.mark.parametrize("precision", ["bf16", "f32"])
 def test_replayed_steps_equal_eager_ones_and_batches_do_not_meet(precision, monkeypatch):
-    """the captured step against the same step queued eagerly; a second batch with shorter rows in the same caches, then the first again"""
+    """the captured step against the same step queued eagerly; a second batch with shorter rows in the same caches, then the first again.
+    Bit for bit, so without the launches around the caches that add floats in the order of their arrival: no split-K GEMMs (the deterministic
+    mode), no one-launch sub-layers (decode_blocks.hip)"""
+    monkeypatch.setattr(modules, "_DECODE_FUSED", False)
+    was = ops.set_deterministic(True)
+    try:
+        replayed_against_eager(precision, monkeypatch)
+    finally:
+        ops.set_deterministic(was)
+
+
+def replayed_against_eager(precision, monkeypatch):
     enc, lens, frames, n = inputs()
     enc2, lens2 = inputs(22)[0] * 3.0, torch.tensor([5, 64, 1], device=DEV)
     res = {}
