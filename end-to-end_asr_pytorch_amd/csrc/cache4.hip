@@ -4,6 +4,8 @@
 // one 32-bit word, the bf16 pair (scale low, mid high): value = mid + scale * code.  scale = bf16((max - min) / 15) and mid = bf16(min + 8
 // scale) put min at code -8 and max at 7 with half a step of room on either side, which is what the two bf16 roundings may use up (mid's is
 // half a step only where |mid| > 256 scale: rows whose level is 17 times their spread).
+#include <type_traits>
+
 #include "asr_common.h"
 
 namespace {
@@ -262,7 +264,7 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
 //
 // What bounds it: HBM for long rows (72 bytes a token and head; 4 rows x 4 heads of 100003 slots, 16 splits: 19.5 us = 4.4 TB/s, + 3.9 us for
 // the join), launch and one chain of loads for a decoding step (32 x 4 rows of 1000 slots: 5.3 us with one query, 7.0 with five), the VALU
-// for chunks (33 queries x 64 rows of up to 2011 slots: 14.7 us; about 110 instructions a tile and 18 a tile and query).
+// and the chain of a tile for many queries (the dense kernel below).
 template <int ND> struct Digits {
     static constexpr float UNIT = ND == 2 ? 127.f * 256.f : 127.f * 65536.f;      // the integer that the largest element becomes
     static constexpr int BIAS = ND == 2 ? 0x80 : 0x8080;                          // u + BIAS, its lower bytes' sign bits inverted: the digits, lowest first
@@ -278,10 +280,10 @@ struct attn4_t {
     const u32x4* kc; const uint32_t* km; const u32x4* vc; const uint32_t* vm;
     void* ctx; float* lse; float* part;
     const int32_t* k_len;
-    int N, h, h_kv, Lq, T, splits, qtiles, rows, waves;
+    int N, h, h_kv, Lq, T, splits, qtiles, per_tile, rows, waves;
 };
 constexpr int PART = 66;      // floats of a partial result: 64 outputs (not divided), reference, sum
-constexpr int MAX_NQ = 4, MAX_WAVES = 8;
+constexpr int MAX_NQ = 4, MAX_WAVES = 8, DENSE_ROW = 68;
 constexpr float NO_REF = -3.4028234663852886e38f;
 
 // position of element k of 16 in the byte order that unpacking leaves: low nibbles of the first word, its high ones, then the second word's
@@ -327,6 +329,11 @@ template <typename OP> __device__ __forceinline__ float wave_all(float v) {     
     x = swap16<OP>(x, x);
     return __builtin_bit_cast(float, row16<OP>(x));
 }
+// over the four rows of 16 lanes: lanes of the same place in their rows
+template <typename OP> __device__ __forceinline__ float over_c(float v) {
+    const uint32_t x = swap32<OP>(__builtin_bit_cast(uint32_t, v), __builtin_bit_cast(uint32_t, v));
+    return __builtin_bit_cast(float, swap16<OP>(x, x));
+}
 // four values at once: row c of the result holds value c's, 9 steps instead of 24
 template <typename OP> __device__ __forceinline__ float wave_four(float v0, float v1, float v2, float v3) {
     const uint32_t a = swap32<OP>(__builtin_bit_cast(uint32_t, v0), __builtin_bit_cast(uint32_t, v2));
@@ -355,6 +362,69 @@ __device__ __forceinline__ void load_tile(tile4_t& t, const u32x4* kc, const u32
     t.vm = vm[tok];
 }
 
+// ---- what the two attention kernels share -----------------------------------------------------------------------------------------------
+struct work4_t { int row, split, n, hk, group, q0, nq; int64_t base; };
+// block -> (row, query tile, split): the query tiles of one stream of keys follow each other at a distance of 8 blocks (one XCD's L2)
+__device__ __forceinline__ bool work_of(const attn4_t& a, int width, work4_t& b) {
+    int stream = blockIdx.x, qt = 0;
+    if (a.qtiles > 1) {
+        const int per8 = 8 * a.qtiles, oct = stream / per8, rest = stream - oct * per8;
+        stream = oct * 8 + (rest & 7);
+        qt = rest >> 3;
+    }
+    if (stream >= a.rows * a.splits) return false;
+    b.row = a.splits == 1 ? stream : stream / a.splits;
+    b.split = stream - b.row * a.splits;
+    b.n = a.h_kv == 1 ? b.row : b.row / a.h_kv;
+    b.hk = b.row - b.n * a.h_kv;
+    b.base = (int64_t)b.row * a.T;
+    b.group = a.h / a.h_kv;
+    b.q0 = qt * a.per_tile;
+    b.nq = min(a.per_tile, b.group * a.Lq - b.q0);
+    return true;
+}
+// the digits of a block's queries, [width][ND][64] in the unpacked operands' order, and behind them [width][2]: the unit of the digits (with the
+// codes' 16), the sum in that unit.  Queries that are not there become zeros.
+template <typename T, int ND> __device__ __forceinline__ float* query_digits(const attn4_t& a, const work4_t& b, int width, unsigned char* sm_q, int wave, int W, int lane) {
+    using D = Digits<ND>;
+    float* sm_qs = reinterpret_cast<float*>(sm_q + width * ND * 64);
+    for (int j = wave; j < width; j += W) {
+        float v = 0.f;
+        if (j < b.nq) {
+            const int qi = b.q0 + j, g = a.Lq == 1 ? qi : qi / a.Lq, i = qi - g * a.Lq;
+            v = to_f32(static_cast<const T*>(a.q)[b.n * a.q_n + (b.hk * b.group + g) * a.q_head + i * a.q_tok + lane]);
+        }
+        const float top = wave_all<MaxPos>(fabsf(v)), sum = wave_all<SumF>(v);
+        const bool some = !(top < 0x1p-100f);      // (below: a query of zeros)
+        const uint32_t u = some ? (uint32_t)((int)__builtin_rintf(v * (D::UNIT / top)) + D::BIAS) ^ D::BIAS : 0u;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) sm_q[(j * ND + d) * 64 + (lane & 48) + unpack_pos(lane & 15)] = (unsigned char)(u >> (8 * d));
+        const float unit = some ? top * (1.f / (16.f * D::UNIT)) : 1.f;
+        if (lane == 0) { sm_qs[2 * j] = unit; sm_qs[2 * j + 1] = some ? sum / unit : 0.f; }
+    }
+    return sm_qs;
+}
+// query q of the block from its waves' parts: sm_o [W][width][pitch] outputs (mid part added), sm_m [W][width][2] references and sums
+template <typename T>
+__device__ __forceinline__ void write_query(const attn4_t& a, const work4_t& b, int q, int width, int pitch, const float* sm_o, const float* sm_m, int W, int lane) {
+    float M = sm_m[q * 2], L = 0.f, o = 0.f;
+    for (int w = 1; w < W; ++w) M = fmaxf(M, sm_m[(w * width + q) * 2]);
+    for (int w = 0; w < W; ++w) {
+        const float f = __builtin_amdgcn_exp2f(sm_m[(w * width + q) * 2] - M);
+        L = __builtin_fmaf(sm_m[(w * width + q) * 2 + 1], f, L);
+        o = __builtin_fmaf(sm_o[(w * width + q) * pitch + lane], f, o);
+    }
+    const int qi = b.q0 + q, g = a.Lq == 1 ? qi : qi / a.Lq, i = qi - g * a.Lq, head = b.hk * b.group + g;
+    if (a.splits == 1) {
+        static_cast<T*>(a.ctx)[(((int64_t)b.n * a.Lq + i) * a.h + head) * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : o / L);
+        if (a.lse && lane == 0) a.lse[((int64_t)b.n * a.h + head) * a.Lq + i] = L == 0.f ? -INFINITY : M + __log2f(L);
+    } else {
+        float* p = a.part + (((int64_t)b.row * b.group * a.Lq + qi) * a.splits + b.split) * PART;
+        p[lane] = o;
+        if (lane == 0) { p[64] = M; p[65] = L; }
+    }
+}
+
 template <typename T, int ND, int NQ, bool CAUSAL>
 __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) {
     using D = Digits<ND>;
@@ -362,45 +432,22 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
     static_assert(NQ <= MAX_NQ, "the rows of lane group c are query c's digits");
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = a.waves, n16 = lane & 15, c = lane >> 4;
-    // block -> (row, query tile, split): the query tiles of one stream of keys follow each other at a distance of 8 blocks (one XCD's L2)
-    int stream = blockIdx.x, qt = 0;
-    if (a.qtiles > 1) {
-        const int per8 = 8 * a.qtiles, oct = stream / per8, rest = stream - oct * per8;
-        stream = oct * 8 + (rest & 7);
-        qt = rest >> 3;
-    }
-    if (stream >= a.rows * a.splits) return;
-    const int row = a.splits == 1 ? stream : stream / a.splits, split = stream - row * a.splits, n = a.h_kv == 1 ? row : row / a.h_kv, hk = row - n * a.h_kv;
-    const int64_t base = (int64_t)row * a.T;
-    const u32x4* kc = a.kc + base * 2;
-    const u32x4* vc = a.vc + base * 2;
-    const uint32_t* km = a.km + base;
-    const uint32_t* vm = a.vm + base;
-    int tile = split * W + wave;
+    work4_t b;
+    if (!work_of(a, NQ, b)) return;
+    const u32x4* kc = a.kc + b.base * 2;
+    const u32x4* vc = a.vc + b.base * 2;
+    const uint32_t* km = a.km + b.base;
+    const uint32_t* vm = a.vm + b.base;
+    int tile = b.split * W + wave;
     tile4_t cur;
     if (tile * 64 < a.T) load_tile(cur, kc, vc, km, vm, tile * 64, a.T - 1, lane);      // (before the row's length is there: inside the cache either way)
-    const int klen = a.k_len ? clampi(a.k_len[n], 0, a.T) : a.T, tiles = (klen + 63) >> 6;
-    if (split > 0 && split * W >= tiles) return;      // (the joining launch knows which splits have a tile)
-    const int group = a.h / a.h_kv, Q = group * a.Lq, q0 = qt * NQ, nq = min(NQ, Q - q0);
+    const int klen = a.k_len ? clampi(a.k_len[b.n], 0, a.T) : a.T, tiles = (klen + 63) >> 6;
+    if (b.split > 0 && b.split * W >= tiles) return;      // (the joining launch knows which splits have a tile)
 
     unsigned char* sm_v = lds + wave * 3072;              // 64 rows of 32 bytes, the halves of rows 8 .. 15 of 16 exchanged
     unsigned char* sm_p = sm_v + 2048;                    // 64 tokens x 16 bytes: the digits of the weights
     unsigned char* sm_q = lds + W * 3072;                 // [NQ][ND][64] digits of the queries
-    float* sm_qs = reinterpret_cast<float*>(sm_q + NQ * ND * 64);      // [NQ][2]: unit of the digits (with the codes' 16), sum in that unit
-    for (int j = wave; j < NQ; j += W) {
-        float v = 0.f;
-        if (j < nq) {
-            const int qi = q0 + j, g = a.Lq == 1 ? qi : qi / a.Lq, i = qi - g * a.Lq;
-            v = to_f32(static_cast<const T*>(a.q)[n * a.q_n + (hk * group + g) * a.q_head + i * a.q_tok + lane]);
-        }
-        const float top = wave_all<MaxPos>(fabsf(v)), sum = wave_all<SumF>(v);
-        const bool some = !(top < 0x1p-100f);      // (below: a query of zeros)
-        const uint32_t u = some ? (uint32_t)((int)__builtin_rintf(v * (D::UNIT / top)) + D::BIAS) ^ D::BIAS : 0u;
-#pragma unroll
-        for (int d = 0; d < ND; ++d) sm_q[(j * ND + d) * 64 + (lane & 48) + unpack_pos(n16)] = (unsigned char)(u >> (8 * d));
-        const float unit = some ? top * (1.f / (16.f * D::UNIT)) : 1.f;
-        if (lane == 0) { sm_qs[2 * j] = unit; sm_qs[2 * j + 1] = some ? sum / unit : 0.f; }
-    }
+    float* sm_qs = query_digits<T, ND>(a, b, NQ, sm_q, wave, W, lane);
     __syncthreads();
     i32x4 qa[PASSES][2];      // [half]: the first or second 16 of a lane's 32 channels
 #pragma unroll
@@ -419,7 +466,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
     for (int q = 0; q < NQ; ++q) {
         unit[q] = sm_qs[2 * q]; qsum[q] = sm_qs[2 * q + 1];
         m[q] = NO_REF; l[q] = 0.f; mv[q] = 0.f;
-        lim[q] = CAUSAL ? klen - (a.Lq - 1) + (q0 + q) % a.Lq : klen;
+        lim[q] = CAUSAL ? klen - (a.Lq - 1) + (b.q0 + q) % a.Lq : klen;
     }
 #pragma unroll
     for (int d = 0; d < 4; ++d) acc[d] = 0.f;
@@ -530,24 +577,166 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
             for (int d = 0; d < 4; ++d) sm_o[(wave * NQ + q) * 64 + d * 16 + n16] = acc[d] + mw;
     }
     __syncthreads();
-    for (int q = wave; q < nq; q += W) {
-        float M = sm_m[q * 2], L = 0.f, o = 0.f;
-        for (int w = 1; w < W; ++w) M = fmaxf(M, sm_m[(w * NQ + q) * 2]);
-        for (int w = 0; w < W; ++w) {
-            const float f = __builtin_amdgcn_exp2f(sm_m[(w * NQ + q) * 2] - M);
-            L = __builtin_fmaf(sm_m[(w * NQ + q) * 2 + 1], f, L);
-            o = __builtin_fmaf(sm_o[(w * NQ + q) * 64 + lane], f, o);
+    for (int q = wave; q < b.nq; q += W) write_query<T>(a, b, q, NQ, 64, sm_o, sm_m, W, lane);
+}
+
+// Many queries: the same products turned round.  K is the A operand (16 tokens a row, 8 bytes of codes a lane), 16 queries the columns, so a lane
+// holds the scores of ONE query for 16 of the tile's 64 tokens - statistics, masks and scales are per lane - and those 16 weights are, as they
+// stand, the lane's share of the PV product's B operand: no LDS between the two products.  V is the A operand (ds_read_b64_tr_b4, its rows read
+// in the order in which the lane holds the tokens), the output [channel, query].  About 390 VALU instructions a tile for 16 queries where the
+// kernel above takes 200 for four; the tokens' scales reach the lanes through LDS.
+constexpr int DENSE_NQ = 16;
+template <typename T, int ND, bool CAUSAL>
+__global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_dense_kernel(attn4_t a) {
+    using D = Digits<ND>;
+    extern __shared__ __align__(16) unsigned char lds[];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = a.waves, n16 = lane & 15, c = lane >> 4;
+    work4_t b;
+    if (!work_of(a, DENSE_NQ, b)) return;
+    const u32x2* kc = reinterpret_cast<const u32x2*>(a.kc + b.base * 2);
+    const u32x4* vc = a.vc + b.base * 2;
+    const uint32_t* km = a.km + b.base;
+    const uint32_t* vm = a.vm + b.base;
+    u32x2 kw[4];
+    u32x4 vw[2];
+    uint32_t kmeta, vmeta;
+    const auto load = [&](int t0, int last) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kw[i] = kc[(unsigned)min(t0 + 16 * i + n16, last) * 4u + c];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) vw[j] = vc[(unsigned)min(t0 + 32 * j + (lane >> 1), last) * 2u + (lane & 1)];
+        const unsigned tok = min(t0 + lane, last);
+        kmeta = km[tok];
+        vmeta = vm[tok];
+    };
+    int tile = b.split * W + wave;
+    if (tile * 64 < a.T) load(tile * 64, a.T - 1);
+    const int klen = a.k_len ? clampi(a.k_len[b.n], 0, a.T) : a.T, tiles = (klen + 63) >> 6;
+    if (b.split > 0 && b.split * W >= tiles) return;
+
+    unsigned char* sm_v = lds + wave * 3072;                            // 64 rows of 32 bytes, the halves of rows 8 .. 15 of 16 exchanged
+    f32x2* sm_k2 = reinterpret_cast<f32x2*>(sm_v + 2048);               // (scale, mid) of K and of V by token
+    f32x2* sm_v2 = sm_k2 + 64;
+    unsigned char* sm_q = lds + W * 3072;
+    float* sm_qs = query_digits<T, ND>(a, b, DENSE_NQ, sm_q, wave, W, lane);
+    __syncthreads();
+    i32x4 qb[ND];
+#pragma unroll
+    for (int d = 0; d < ND; ++d) qb[d] = *reinterpret_cast<const i32x4*>(sm_q + (n16 * ND + d) * 64 + c * 16);
+    const float unit = sm_qs[2 * n16], qsum = sm_qs[2 * n16 + 1];
+    const int lim = CAUSAL ? klen - (a.Lq - 1) + (b.q0 + n16) % a.Lq : klen, all_see = CAUSAL ? klen - (a.Lq - 1) : klen;
+    float m = NO_REF, l = 0.f, mv = 0.f;
+    f32x4 acc[4];
+#pragma unroll
+    for (int d = 0; d < 4; ++d) acc[d] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    const int step = a.splits * W;
+    for (; tile < tiles; tile += step) {
+        const int t0 = tile * 64;
+        i32x4 ku[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ku[i] = unpack16(kw[i][0], kw[i][1]);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int r = 32 * j + (lane >> 1);
+            *reinterpret_cast<u32x4*>(sm_v + r * 32 + (((lane & 1) ^ ((r >> 3) & 1)) << 4)) = vw[j];
         }
-        const int qi = q0 + q, g = a.Lq == 1 ? qi : qi / a.Lq, i = qi - g * a.Lq, head = hk * group + g;
-        if (a.splits == 1) {
-            static_cast<T*>(a.ctx)[(((int64_t)n * a.Lq + i) * a.h + head) * 64 + lane] = from_f32<T>(L == 0.f ? 0.f : o / L);
-            if (a.lse && lane == 0) a.lse[((int64_t)n * a.h + head) * a.Lq + i] = L == 0.f ? -INFINITY : M + __log2f(L);
-        } else {
-            float* p = a.part + (((int64_t)row * Q + qi) * a.splits + split) * PART;
-            p[lane] = o;
-            if (lane == 0) { p[64] = M; p[65] = L; }
-        }
+        const bool live = t0 + lane < klen;      // (what is behind the last token may be anything)
+        if (!live) kmeta = vmeta = 0u;
+        sm_k2[lane] = f32x2{meta_scale(kmeta), meta_mid(kmeta)};
+        sm_v2[lane] = f32x2{meta_scale(vmeta), meta_mid(vmeta)};
+        if (tile + step < tiles) load((tile + step) * 64, klen - 1);
+        wave_lds_fence();
+        const auto work = [&](auto masked) {
+            float s[4][4], e[4][4], top = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                i32x4 dot[ND];
+#pragma unroll
+                for (int d = 0; d < ND; ++d) dot[d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(ku[i], qb[d], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {      // tokens 16 i + 4 c + r, + 1
+                    const f32x4 k2 = *reinterpret_cast<const f32x4*>(sm_k2 + 16 * i + 4 * c + r);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v = __builtin_fmaf(D::join(dot[0][r + h], dot[1][r + h], dot[ND - 1][r + h]), k2[2 * h], k2[2 * h + 1] * qsum);
+                        if (decltype(masked)::value) v = t0 + 16 * i + 4 * c + r + h < lim ? v : -INFINITY;
+                        s[i][r + h] = v;
+                        e[i][r + h] = __builtin_fmaf(v, unit, -m);
+                        top = fmaxf(top, e[i][r + h]);
+                    }
+                }
+            }
+            if (__builtin_amdgcn_ballot_w64(top > 32.f)) {
+                float big = s[0][0];
+#pragma unroll
+                for (int x = 1; x < 16; ++x) big = __builtin_elementwise_maximum(big, s[x >> 2][x & 3]);
+                const float mn = __builtin_elementwise_maximum(m, over_c<MaxF>(big) * unit), al = __builtin_amdgcn_exp2f(m - mn);
+                m = mn; l *= al; mv *= al;
+#pragma unroll
+                for (int d = 0; d < 4; ++d) acc[d] *= al;
+#pragma unroll
+                for (int x = 0; x < 16; ++x) e[x >> 2][x & 3] = __builtin_fmaf(s[x >> 2][x & 3], unit, -m);
+            }
+            uint32_t most = 0u;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; r += 2) {
+                    const f32x4 v2 = *reinterpret_cast<const f32x4*>(sm_v2 + 16 * i + 4 * c + r);
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float p = __builtin_amdgcn_exp2f(e[i][r + h]);
+                        const bool seen = !decltype(masked)::value || t0 + 16 * i + 4 * c + r + h < lim;      // (0 * NaN of a token that another query sees)
+                        l += p;
+                        mv = __builtin_fmaf(p, seen ? v2[2 * h + 1] : 0.f, mv);
+                        s[i][r + h] = p * (seen ? v2[2 * h] : 0.f);
+                        most = max(most, __builtin_bit_cast(uint32_t, s[i][r + h]));
+                    }
+                }
+            const float mo = over_c<MaxPos>(__builtin_bit_cast(float, most));
+            const float inv = mo > 1e-30f ? D::UNIT * __builtin_amdgcn_rcpf(mo) : 0.f, wunit = mo * (1.f / (16.f * D::UNIT));
+            i32x4 pb[ND];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t u[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    u[r] = ND == 2 ? __builtin_bit_cast(uint32_t, __builtin_fmaf(s[i][r], inv, 12582912.f + D::BIAS)) : (uint32_t)__builtin_fmaf(s[i][r], inv, D::BIAS + 0.5f);
+                const uint32_t t01 = __builtin_amdgcn_perm(u[1], u[0], 0x05010400u), t23 = __builtin_amdgcn_perm(u[3], u[2], 0x05010400u);
+                pb[0][i] = (int)(__builtin_amdgcn_perm(t23, t01, 0x05040100u) ^ 0x80808080u);
+                pb[1][i] = (int)(__builtin_amdgcn_perm(t23, t01, 0x07060302u) ^ (ND == 3 ? 0x80808080u : 0u));
+                if (ND == 3) pb[ND - 1][i] = (int)(__builtin_amdgcn_perm(u[1], u[0], 0x0c0c0602u) | __builtin_amdgcn_perm(u[3], u[2], 0x06020c0cu));
+            }
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                // lane k of group c reads the row of the token that is element k of the unpacked operand: byte r of word i = token 16 i + 4 c + r
+                const int row = 16 * ((n16 & 1) + 2 * (n16 >> 3)) + 4 * c + ((n16 >> 1) & 3);
+                const i32x2 vt = __builtin_amdgcn_ds_read_tr4_b64_v2i32((lds_i32x2*)((__attribute__((address_space(3))) unsigned char*)sm_v + row * 32 +
+                                                                                      (((d >> 1) ^ ((row >> 3) & 1)) << 4) + (d & 1) * 8));
+                const i32x4 va = unpack16((uint32_t)vt[0], (uint32_t)vt[1]);
+                i32x4 o[ND];
+#pragma unroll
+                for (int x = 0; x < ND; ++x) o[x] = __builtin_amdgcn_mfma_i32_16x16x64_i8(va, pb[x], i32x4{0, 0, 0, 0}, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) acc[d][r] = __builtin_fmaf(D::join(o[0][r], o[1][r], o[ND - 1][r]), wunit, acc[d][r]);
+            }
+        };
+        if (t0 + 64 <= all_see) work(std::false_type{});
+        else work(std::true_type{});
+        wave_lds_fence();
     }
+
+    __syncthreads();
+    float* sm_o = reinterpret_cast<float*>(lds);                      // [W][16][DENSE_ROW], 68 floats a row: 16 lanes' 16-byte stores meet no bank twice
+    float* sm_m = sm_o + W * DENSE_NQ * DENSE_ROW;                    // [W][16][2]
+    l = over_c<SumF>(l);
+    mv = over_c<SumF>(mv);
+#pragma unroll
+    for (int d = 0; d < 4; ++d) *reinterpret_cast<f32x4*>(sm_o + (wave * DENSE_NQ + n16) * DENSE_ROW + 16 * d + 4 * c) = acc[d] + mv;
+    if (c == 0) { sm_m[(wave * DENSE_NQ + n16) * 2] = m; sm_m[(wave * DENSE_NQ + n16) * 2 + 1] = l; }
+    __syncthreads();
+    for (int q = wave; q < b.nq; q += W) write_query<T>(a, b, q, DENSE_NQ, DENSE_ROW, sm_o, sm_m, W, lane);
 }
 
 // joins the splits of one query: 8 waves of up to MAX_SPLITS / 8 partial results each, all loads in front
@@ -595,22 +784,30 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void cache4_join_kernel(attn4_t a)
 }
 
 // How a call is cut.  Times in us, bf16, graph replays, keys cold where they do not fit the caches.
-//   queries a block   up to 4, evenly: eight need 184 VGPRs instead of 106 and lose at every size (5 queries x 128 rows x 1000 slots 8.4 against
-//                     7.1, 33 queries x 64 rows x 2011 slots 17.0 against 14.7)
+//   kernel            the dense one does half the work a query and has the longer chain a tile: from 9 queries a key head up, where there is work
+//                     for many waves - 12 tiles of four queries a SIMD, or four blocks a CU.  64 rows x 2011 slots: 33 queries 12.0 against 15.5, 128
+//                     queries 20.6 against 32.0, but 16 queries 12.3 against 8.7; 640 rows x 101 slots: 16 queries 11.0 against 12.7, 8 queries 9.0
+//                     against 8.0; 8 rows x 20000 slots: 64 queries 17.7 against 24.1, 16 queries 13.1 against 12.4
+//   queries a block   up to 4 (16 in the dense kernel), evenly: eight in the first kernel need 184 VGPRs instead of 106 and lose at every size (5
+//                     queries x 128 rows x 1000 slots 8.4 against 7.1)
 //   waves             one per tile of 64 slots up to 8; 4 where more blocks than CUs make a CU take two anyway (300 rows x 2000 slots 12.6 with 8,
-//                     11.6 with 4; 230 rows 8.8 and 9.3; 128 rows x 1000 slots 5.8 with 8, 5.9 with 4, 7.7 with 2)
+//                     11.6 with 4; 230 rows 8.8 and 9.3; 128 rows x 1000 slots 5.8 with 8, 5.9 with 4, 7.7 with 2).  The dense kernel's waves also
+//                     share the queries' digits: never fewer for few tiles (640 rows x 101 slots: 11.0 with 4, 12.4 with 2)
 //   splits            where a wave would walk more than 4 tiles and there are no more than 128 blocks: as many as fill 256 CUs with a block each,
 //                     two tiles a wave at least (16 rows x 100003 slots: 1 split 168, 16 splits 26.6, 32 splits 27.8; 4 rows: 32 splits 11.6, 20
 //                     13.4).  Below that the second launch costs more than it gives (20 rows x 777 slots 4.9 against 6.4).
-struct plan_t { int nq, qtiles, splits, waves; };
+struct plan_t { int nq, qtiles, splits, waves; bool dense; };
 plan_t attn_plan(int rows, int Q, int T) {
     plan_t p;
-    p.qtiles = (Q + MAX_NQ - 1) / MAX_NQ;
-    p.nq = (Q + p.qtiles - 1) / p.qtiles;
     const int tiles = (T + 63) / 64;
+    const int64_t fours = (int64_t)rows * ((Q + MAX_NQ - 1) / MAX_NQ);
+    p.dense = Q > 8 && (fours * tiles >= 12 * 1024 || fours > 1024);
+    const int width = p.dense ? DENSE_NQ : MAX_NQ;
+    p.qtiles = (Q + width - 1) / width;
+    p.nq = (Q + p.qtiles - 1) / p.qtiles;
     const int64_t blocks = (int64_t)rows * p.qtiles;
-    const int most = blocks > 256 ? 4 : 8;
-    p.waves = 1;
+    const int most = blocks > 256 ? 4 : MAX_WAVES;
+    p.waves = p.dense ? most : 1;
     while (p.waves < most && p.waves < tiles) p.waves *= 2;
     p.splits = 1;
     if (tiles > 32 && blocks <= 128) {
@@ -621,16 +818,21 @@ plan_t attn_plan(int rows, int Q, int T) {
 }
 
 template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, const plan_t& p, bool causal) {
-    const size_t work = (size_t)p.waves * 3072 + p.nq * (ND * 64 + 8), join = (size_t)p.waves * p.nq * 66 * 4;
-    const size_t lds = work > join ? work : join;
+    const int width = p.dense ? DENSE_NQ : p.nq, pitch = p.dense ? DENSE_ROW : 64;
+    const size_t work = (size_t)p.waves * 3072 + width * (ND * 64 + 8), join = (size_t)p.waves * width * (pitch + 2) * 4;
+    const size_t lds = work > join ? work : join;      // (at most 35.8 KiB)
     const int64_t streams = (int64_t)a.rows * a.splits;
     const dim3 grid((unsigned)(a.qtiles == 1 ? streams : (streams + 7) / 8 * 8 * a.qtiles)), block(p.waves * 64);
-#define ASR_C4(NQ)                                                                                      \
-    case NQ:                                                                                            \
-        if (causal) hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, true>), grid, block, lds, s, a);  \
-        else hipLaunchKernelGGL((cache4_attn_kernel<T, ND, NQ, false>), grid, block, lds, s, a);        \
-        break;
-    switch (p.nq) { ASR_C4(1) ASR_C4(2) ASR_C4(3) ASR_C4(4) }
+#define ASR_C4(...)                                                                                     \
+    do {                                                                                                \
+        if (causal) hipLaunchKernelGGL((__VA_ARGS__, true>), grid, block, lds, s, a);                   \
+        else hipLaunchKernelGGL((__VA_ARGS__, false>), grid, block, lds, s, a);                         \
+    } while (0)
+    if (p.dense) ASR_C4(cache4_attn_dense_kernel<T, ND);
+    else if (p.nq == 1) ASR_C4(cache4_attn_kernel<T, ND, 1);
+    else if (p.nq == 2) ASR_C4(cache4_attn_kernel<T, ND, 2);
+    else if (p.nq == 3) ASR_C4(cache4_attn_kernel<T, ND, 3);
+    else ASR_C4(cache4_attn_kernel<T, ND, 4);
 #undef ASR_C4
     ASR_LAUNCH_CHECK("cache4_attention");
     if (a.splits > 1) {
@@ -744,7 +946,7 @@ extern "C" int asr_cache4_attention(void* stream, const void* q, int dtype, int6
     ASR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asr_aligned(workspace, 4)), ASR_ERR_ARG, "cache4_attention: workspace of %lld bytes needed, %lld given",
                 (long long)need, (long long)(workspace ? workspace_bytes : 0));
     attn4_t a{q, s_n, s_head, s_tok, static_cast<const u32x4*>(k_codes), static_cast<const uint32_t*>(k_meta), static_cast<const u32x4*>(v_codes),
-              static_cast<const uint32_t*>(v_meta), ctx, lse, static_cast<float*>(workspace), k_len, N, h, h_kv, Lq, T, p.splits, p.qtiles,
+              static_cast<const uint32_t*>(v_meta), ctx, lse, static_cast<float*>(workspace), k_len, N, h, h_kv, Lq, T, p.splits, p.qtiles, p.nq,
               N * h_kv, p.waves};
     hipStream_t s = static_cast<hipStream_t>(stream);
     return dtype == ASR_BF16 ? attn_launch<bf16_t, 2>(s, a, p, causal != 0) : attn_launch<float, 3>(s, a, p, causal != 0);

@@ -371,6 +371,47 @@ def test_attention_query_strides():
     assert torch.equal(want, ops.cache4_attention(wide[:, :, 1].transpose(1, 2), kc, vc)[0])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N,h,h_kv,Lq,T", [(64, 2, 2, 33, 130), (140, 8, 1, 4, 65), (12, 8, 8, 33, 1300), (400, 4, 1, 3, 70), (2, 2, 1, 50, 20000),
+                                           (600, 2, 2, 9, 40)])
+def test_attention_many_queries(N, h, h_kv, Lq, T, dtype):
+    """enough queries and rows for the dense kernel (16 queries a block, a lane a query: more than 8 a key head, and more than 1024 groups of four
+    or 12 288 tiles of them; the longest with split keys): the first, the last and two rows between against the reference"""
+    g = torch.Generator().manual_seed(N + T)
+    q, kc, vc = make(g, N, h, h_kv, Lq, T, dtype)
+    lens = [max(0, T - (n * 29) % (T + 1)) if n else T for n in range(N)]
+    for causal in (False, True):
+        got, lse = ops.cache4_attention(q, kc, vc, k_len=i32(*lens), causal=causal, need_lse=True)
+        for n in sorted({0, 1, N // 2, N - 1}):
+            one = lambda c: ops.Cache4(c.codes[n:n + 1].contiguous(), c.meta[n:n + 1].contiguous())  # noqa: E731
+            want, wl, tol, lt = reference(q[n:n + 1], one(kc), one(vc), [lens[n]], causal, dtype)
+            d = (got[n:n + 1].double().cpu() - want).abs()
+            assert bool((d <= tol).all()), "row %d: worst %.3g of its tolerance" % (n, float((d / tol).max()))
+            seen, l = ~torch.isinf(wl), lse[n:n + 1].double().cpu()
+            assert torch.equal(torch.isinf(l), ~seen) and bool(((l - wl).abs()[seen] <= lt[seen]).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_masked_slots_many_queries(dtype):
+    """the dense kernel: anything behind the last token; a NaN token that only the last queries see"""
+    g = torch.Generator().manual_seed(77)
+    N, T, Lq = 110, 300, 20
+    q, kc, vc = make(g, N, 2, 2, Lq, T, dtype)
+    lens = [T - 20 - n % 64 for n in range(N)]
+    want = [ops.cache4_attention(q, kc, vc, k_len=i32(*lens), causal=causal)[0] for causal in (False, True)]
+    for c in (kc, vc):
+        for n, ln in enumerate(lens):
+            c.meta[n, :, ln:] = torch.tensor([math.nan, math.inf], dtype=torch.bfloat16, device=DEV)
+            c.codes[n, :, ln:] = 0x5A
+    for causal in (False, True):
+        assert torch.equal(ops.cache4_attention(q, kc, vc, k_len=i32(*lens), causal=causal)[0], want[causal])
+    for c in (kc, vc):
+        for n, ln in enumerate(lens):
+            c.meta[n, :, ln - 3] = math.nan
+    got = ops.cache4_attention(q, kc, vc, k_len=i32(*lens), causal=True)[0]
+    assert torch.equal(got[:, :Lq - 3], want[1][:, :Lq - 3]) and bool(got[:, Lq - 3:].isnan().all())
+
+
 def test_repeatable():
     g = torch.Generator().manual_seed(6)
     q, kc, vc = make(g, 2, 4, 2, 5, 6000, torch.bfloat16)
