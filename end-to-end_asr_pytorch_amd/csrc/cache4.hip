@@ -1,8 +1,8 @@
 // K / V cache held in 4 bits: quantising put, reading back, attention over it, re-gathering by parent hypothesis (asr_hip.h: asr_cache4_*).
 //
 // A row of 64 values (one head of one token) is 32 bytes of signed codes - byte j: value 2j in the low nibble, 2j + 1 in the high one - and
-// one 32-bit word, the bf16 pair (scale low, mid high): value = mid + scale * code.  scale = bf16((max - min) / 15) and mid = bf16(min + 8
-// scale) put min at code -8 and max at 7 with half a step of room on either side, which is what the two bf16 roundings may use up (mid's is
+// one 32-bit word, the bf16 pair (scale low, mid high): value = mid + scale * code.  scale = bf16((max - min) * (1/15)) and mid = bf16(min
+// + 8 scale) put min at code -8 and max at 7 with half a step of room on either side, which is what the two bf16 roundings may use up (mid's is
 // half a step only where |mid| > 256 scale: rows whose level is 17 times their spread).
 #include <type_traits>
 
@@ -87,8 +87,7 @@ template <typename T> __device__ __forceinline__ u32x2 quantise16(const float (&
     hi = __builtin_elementwise_maximum(hi, dpp_f<0x4E>(hi));
     const float span = hi - lo;
     const bool fine = span < INFINITY;
-    // (span / 15 rounded to nearest: 1.f / 15.f is the reciprocal rounded to nearest, so one corrected step is the correctly rounded quotient)
-    const float sc = span < 0x1p-100f || !fine ? 0.f : (float)(bf16_t)quotient(span, 15.f, 1.f / 15.f);
+    const float sc = span < 0x1p-100f || !fine ? 0.f : (float)(bf16_t)(span * (1.f / 15.f));      // (the format: a product, not a quotient)
     const float mid = (float)(bf16_t)(lo + 8.f * sc);
     meta = fine ? bf16_bits(sc) | (bf16_bits(mid) << 16) : 0x7fc07fc0u;
     if (sc == 0.f) return u32x2{0u, 0u};

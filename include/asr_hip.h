@@ -645,7 +645,7 @@ int asr_beam_advance(void* stream, int32_t* state, int32_t* k_len, int N, const 
  *   codes  uint8 [n_kv, N, h, Tmax, 32]   signed 4-bit codes: byte j holds value 2j in its low nibble and value 2j + 1 in its high one
  *   meta   bf16  [n_kv, N, h, Tmax, 2]    (scale >= 0, mid);  the value a code stands for is mid + scale * code
  * Both contiguous; codes start on 16 bytes, meta on 4.  4.5 bits a value.  Quantising (asr_cache4_put), per slot:
- *   span = max - min (f32);  scale = bf16(span / 15), 0 where span < 2^-100;  mid = bf16(min + 8 * scale)
+ *   span = max - min;  scale = bf16(span * (1/15)), 0 where span < 2^-100;  mid = bf16(min + 8 * scale);  all in f32, 1/15 rounded to it
  *   code = (x - mid) / scale rounded to the nearest integer, ties to even - decided exactly, not from a rounded quotient -, cut to [-8, 7]
  *   (0 where scale is 0: a constant slot reads back as bf16 of its value).  A slot with a NaN or an infinity, or whose span overflows f32,
  *   gets scale = mid = NaN and reads back as NaN; where it is masked it is never looked at.

@@ -14,6 +14,7 @@ from asr_amd import ops
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
 LOG2E = 1.4426950408889634
+FIFTEENTH = torch.tensor(1.0) / torch.tensor(15.0)                       # in f32, as the format has it
 UNIT = {torch.bfloat16: 127 * 256, torch.float32: 127 * 65536}      # what the largest element becomes in digits of base 256
 
 
@@ -26,7 +27,7 @@ def quantise(x):
     x = x.double()
     lo, hi = x.amin(-1), x.amax(-1)
     span = (hi.float() - lo.float())
-    scale = torch.where(span < 2.0 ** -100, torch.zeros_like(span), span / 15.0).bfloat16().double()
+    scale = torch.where(span < 2.0 ** -100, torch.zeros_like(span), span * FIFTEENTH.to(span.device)).bfloat16().double()
     mid = (lo.float() + 8.0 * scale.float()).bfloat16().double()
     bad = ~(span < math.inf)
     q = (x - mid[..., None]) / scale[..., None]
@@ -204,6 +205,19 @@ def test_empty_calls():
     assert int(ctx.abs().sum()) == 0 and bool(torch.isinf(lse).all())
     none = ops.Cache4.empty(2, 0, 4, 8, DEV)
     assert ops.cache4_attention(torch.zeros(0, 4, 1, 64, device=DEV), none[0], none[1])[0].shape == (0, 1, 256)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_rows(dtype):
+    """a quarter of a million rows, spans over twelve octaves: scale and mid of every row (one f32 ulp in the span's multiple moves a bf16 scale in
+    about one row of 2^16)"""
+    g = torch.Generator().manual_seed(41)
+    x = torch.randn(4, 16, 4, 1024, 64, generator=g) * torch.exp2(12 * torch.rand(4, 16, 4, 1024, 1, generator=g) - 6)
+    x = (x + torch.randn(4, 16, 4, 1024, 1, generator=g)).to(dtype).to(DEV)
+    c = ops.Cache4.empty(4, 16, 4, 1024, DEV)
+    ops.cache4_put(c, x)
+    codes, meta = pack(*quantise(x))
+    assert torch.equal(c.meta, meta) and torch.equal(c.codes, codes)
 
 
 # ---- attention -------------------------------------------------------------------------------------------------------------------------
