@@ -841,18 +841,24 @@ template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, c
     return 0;
 }
 
+// a * b * c <= most, for sizes whose product may pass 64 bits
+bool fits(int64_t a, int64_t b, int64_t c, int64_t most) { return a <= most && b <= most / a && c <= most / (a * b); }
+constexpr int64_t MAX_BLOCKS = (1 << 24) - 1;      // of 256 threads: a launch holds fewer than 2^32
+constexpr int64_t MAX_QUERIES = (1 << 24) - 1;     // (a block each of up to 256 threads, or more queries a block)
+
 int slots_plan(const char* name, int lanes, slots_t& s, int64_t& blocks, int n_kv, int N, int h, int L, int Tmax, const int32_t* pos, int pos_stride,
                const int32_t* n_tok) {
     ASR_REQUIRE(n_kv > 0 && N > 0 && h > 0 && L > 0 && Tmax > 0, ASR_ERR_ARG, "%s: bad sizes (n_kv=%d N=%d h=%d L=%d Tmax=%d)", name, n_kv, N, h, L, Tmax);
     ASR_REQUIRE(Tmax <= CACHE4_MAX_T && L <= CACHE4_MAX_T, ASR_ERR_UNSUPPORTED, "%s: more than 2^24 slots", name);
     ASR_REQUIRE(pos_stride == 0 || pos_stride == 1, ASR_ERR_ARG, "%s: pos_stride is 0 (one position for all rows) or 1", name);
+    ASR_REQUIRE(fits(n_kv, N, h, INT32_MAX - 64), ASR_ERR_UNSUPPORTED, "%s: too many rows", name);
     const int64_t rows = (int64_t)n_kv * N * h;
     const int groups_log2 = lanes == 4 ? 6 : 5;      // rows of 64 values side by side in a block of 256 threads
     int lg = 0;
     while (lg < groups_log2 && (1 << lg) < L) ++lg;
     const int rb_log2 = groups_log2 - lg, iter = 4, chunks = (int)((L + ((int64_t)iter << lg) - 1) / ((int64_t)iter << lg));
     blocks = (rows + (1 << rb_log2) - 1) / (1 << rb_log2) * chunks;
-    ASR_REQUIRE(rows <= INT32_MAX - 64 && blocks <= INT32_MAX, ASR_ERR_UNSUPPORTED, "%s: too many rows", name);
+    ASR_REQUIRE(blocks <= MAX_BLOCKS, ASR_ERR_UNSUPPORTED, "%s: too many rows", name);
     s = slots_t{pos, n_tok, pos_stride, N, h, L, Tmax, lg, rb_log2, iter, chunks, (int)rows};
     return 0;
 }
@@ -910,8 +916,8 @@ extern "C" int asr_cache4_reorder(void* stream, const void* codes, const void* m
     ASR_REQUIRE((codes == out_codes) == (meta == out_meta), ASR_ERR_ARG, "cache4_reorder: in place means codes and meta both");
     ASR_REQUIRE(asr_aligned(codes, 16) && asr_aligned(out_codes, 16) && asr_aligned(meta, 4) && asr_aligned(out_meta, 4), ASR_ERR_ALIGN, "cache4_reorder: alignment");
     const int chunks_codes = (2 * Tmax + 255) / 256, chunks_meta = (Tmax + 255) / 256;
-    const int64_t blocks = (int64_t)n_kv * B * h * (chunks_codes + chunks_meta);
-    ASR_REQUIRE(blocks <= INT32_MAX, ASR_ERR_UNSUPPORTED, "cache4_reorder: too many rows");
+    ASR_REQUIRE(fits(n_kv, B, h, MAX_BLOCKS / (chunks_codes + chunks_meta)), ASR_ERR_UNSUPPORTED, "cache4_reorder: too many rows");
+    const int blocks = n_kv * B * h * (chunks_codes + chunks_meta);
     hipStream_t hs = static_cast<hipStream_t>(stream);
 #define ASR_C4(BEAM)                                                                                                                                     \
     hipLaunchKernelGGL((cache4_reorder_kernel<BEAM>), dim3((unsigned)blocks), dim3(256), 0, hs, static_cast<const u32x4*>(codes), static_cast<const uint32_t*>(meta), \
@@ -925,7 +931,7 @@ extern "C" int asr_cache4_reorder(void* stream, const void* codes, const void* m
 }
 
 extern "C" int64_t asr_cache4_attention_workspace_bytes(int N, int h, int h_kv, int Lq, int T) {
-    if (N <= 0 || h_kv <= 0 || h <= 0 || h % h_kv || Lq <= 0 || T <= 0 || (int64_t)N * h_kv > INT32_MAX || (int64_t)(h / h_kv) * Lq > INT32_MAX) return 0;
+    if (N <= 0 || h_kv <= 0 || h <= 0 || h % h_kv || Lq <= 0 || T <= 0 || T > CACHE4_MAX_T || !fits(N, h, Lq, MAX_QUERIES)) return 0;      // (no call that is taken)
     const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T);
     return p.splits == 1 ? 0 : (int64_t)N * h * Lq * p.splits * PART * 4;
 }
@@ -937,7 +943,7 @@ extern "C" int asr_cache4_attention(void* stream, const void* q, int dtype, int6
     ASR_REQUIRE(dtype == ASR_F32 || dtype == ASR_BF16, ASR_ERR_ARG, "cache4_attention: dtype %d (ASR_F32 or ASR_BF16)", dtype);
     ASR_REQUIRE(N > 0 && h > 0 && h_kv > 0 && Lq > 0 && T > 0 && h % h_kv == 0, ASR_ERR_ARG, "cache4_attention: bad sizes (N=%d h=%d h_kv=%d Lq=%d T=%d)", N, h, h_kv, Lq, T);
     ASR_REQUIRE(T <= CACHE4_MAX_T, ASR_ERR_UNSUPPORTED, "cache4_attention: more than 2^24 slots");
-    ASR_REQUIRE((int64_t)N * h * Lq <= INT32_MAX / 128, ASR_ERR_UNSUPPORTED, "cache4_attention: more than 2^24 queries");
+    ASR_REQUIRE(fits(N, h, Lq, MAX_QUERIES), ASR_ERR_UNSUPPORTED, "cache4_attention: more than 2^24 queries");
     ASR_REQUIRE(asr_aligned(q, dtype == ASR_F32 ? 4 : 2) && asr_aligned(ctx, dtype == ASR_F32 ? 4 : 2) && asr_aligned(k_codes, 16) && asr_aligned(v_codes, 16) && asr_aligned(k_meta, 4) && asr_aligned(v_meta, 4),
                 ASR_ERR_ALIGN, "cache4_attention: codes start on 16 bytes, meta on 4, q and ctx on their elements");
     const plan_t p = attn_plan(N * h_kv, h / h_kv * Lq, T);

@@ -113,6 +113,32 @@ def test_library_refuses_before_it_launches():
     assert L.asr_cache4_attention_workspace_bytes(1, 4, 4, 1, 8) == 0 and L.asr_cache4_attention_workspace_bytes(1, 4, 3, 1, 8) == 0
 
 
+def test_library_refuses_sizes_that_no_launch_holds():
+    """a launch holds fewer than 2^32 threads, 2^24 blocks of 256; products of sizes that pass 64 bits are too many as well, not few"""
+    L = asr_amd.lib()
+    p, top = ctypes.c_void_p(64), (1 << 31) - 1
+
+    def put(*sizes):
+        return L.asr_cache4_put(None, p, 1, 0, 0, 0, 64, p, p, None, 0, None, *sizes)
+
+    def get(*sizes):
+        return L.asr_cache4_get(None, p, p, p, 1, 0, 0, 0, 64, None, 0, None, *sizes)
+
+    for call in (put, get):
+        assert call(1, 1 << 10, 1 << 10, 1 << 13, 1 << 13) == -3 and b"too many rows" in L.asr_last_error()      # 2^20 rows of 32 or 64 blocks
+        assert call(1, 1 << 15, 1 << 15, 1, 1) == -3 and call(top, top, top, 1, 8) == -3 and call(1 << 30, 1 << 30, 16, 1, 8) == -3      # (2^64 rows)
+
+    def reorder(n_kv, B, h, T):
+        return L.asr_cache4_reorder(None, p, p, p, p, p, p, n_kv, B, 2, h, T)
+    assert reorder(1, 1 << 12, 1 << 10, 1 << 9) == -3 and reorder(top, top, top, 8) == -3 and reorder(1 << 30, 1 << 30, 16, 8) == -3
+
+    def attn(N, h, h_kv, Lq):
+        return L.asr_cache4_attention(None, p, 1, 0, 0, 0, p, p, p, p, p, None, N, h, h_kv, Lq, 8, None, 0, None, 0)
+    assert attn(1 << 30, 1 << 30, 1, 16) == -3 and attn(top, top, top, top) == -3 and attn(1 << 24, 1, 1, 1) == -3
+    size = L.asr_cache4_attention_workspace_bytes
+    assert size(1, 1 << 30, 1, 1, 1 << 24) == 0 and size(1 << 30, 1 << 30, 1 << 30, 16, 1 << 24) == 0 and size(1, 4, 4, 1, (1 << 24) + 1) == 0      # (no call that is taken)
+
+
 def test_header_revision():
     assert asr_amd.lib().asr_version() >= 103
     assert "103 = asr_cache4_* added" in open(_lib.HEADER).read()
