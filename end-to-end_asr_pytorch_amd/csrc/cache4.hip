@@ -283,6 +283,7 @@ struct attn4_t {
 };
 constexpr int PART = 66;      // floats of a partial result: 64 outputs (not divided), reference, sum
 constexpr int MAX_NQ = 4, MAX_WAVES = 8, DENSE_ROW = 68;
+constexpr int TILE_V = 64 * 32, WAVE_LDS = TILE_V + 64 * 16;      // LDS bytes of a wave: a tile's codes of V; 16 bytes a token behind them
 constexpr float NO_REF = -3.4028234663852886e38f;
 
 // position of element k of 16 in the byte order that unpacking leaves: low nibbles of the first word, its high ones, then the second word's
@@ -443,9 +444,9 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
     const int klen = a.k_len ? clampi(a.k_len[b.n], 0, a.T) : a.T, tiles = (klen + 63) >> 6;
     if (b.split > 0 && b.split * W >= tiles) return;      // (the joining launch knows which splits have a tile)
 
-    unsigned char* sm_v = lds + wave * 3072;              // 64 rows of 32 bytes, the halves of rows 8 .. 15 of 16 exchanged
-    unsigned char* sm_p = sm_v + 2048;                    // 64 tokens x 16 bytes: the digits of the weights
-    unsigned char* sm_q = lds + W * 3072;                 // [NQ][ND][64] digits of the queries
+    unsigned char* sm_v = lds + wave * WAVE_LDS;              // 64 rows of 32 bytes, the halves of rows 8 .. 15 of 16 exchanged
+    unsigned char* sm_p = sm_v + TILE_V;                    // 64 tokens x 16 bytes: the digits of the weights
+    unsigned char* sm_q = lds + W * WAVE_LDS;                 // [NQ][ND][64] digits of the queries
     float* sm_qs = query_digits<T, ND>(a, b, NQ, sm_q, wave, W, lane);
     __syncthreads();
     i32x4 qa[PASSES][2];      // [half]: the first or second 16 of a lane's 32 channels
@@ -613,10 +614,10 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_dense_kernel(attn4
     const int klen = a.k_len ? clampi(a.k_len[b.n], 0, a.T) : a.T, tiles = (klen + 63) >> 6;
     if (b.split > 0 && b.split * W >= tiles) return;
 
-    unsigned char* sm_v = lds + wave * 3072;                            // 64 rows of 32 bytes, the halves of rows 8 .. 15 of 16 exchanged
-    f32x2* sm_k2 = reinterpret_cast<f32x2*>(sm_v + 2048);               // (scale, mid) of K and of V by token
+    unsigned char* sm_v = lds + wave * WAVE_LDS;                            // 64 rows of 32 bytes, the halves of rows 8 .. 15 of 16 exchanged
+    f32x2* sm_k2 = reinterpret_cast<f32x2*>(sm_v + TILE_V);               // (scale, mid) of K and of V by token
     f32x2* sm_v2 = sm_k2 + 64;
-    unsigned char* sm_q = lds + W * 3072;
+    unsigned char* sm_q = lds + W * WAVE_LDS;
     float* sm_qs = query_digits<T, ND>(a, b, DENSE_NQ, sm_q, wave, W, lane);
     __syncthreads();
     i32x4 qb[ND];
@@ -818,7 +819,7 @@ plan_t attn_plan(int rows, int Q, int T) {
 
 template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, const plan_t& p, bool causal) {
     const int width = p.dense ? DENSE_NQ : p.nq, pitch = p.dense ? DENSE_ROW : 64;
-    const size_t work = (size_t)p.waves * 3072 + width * (ND * 64 + 8), join = (size_t)p.waves * width * (pitch + 2) * 4;
+    const size_t work = (size_t)p.waves * WAVE_LDS + width * (ND * 64 + 8), join = (size_t)p.waves * width * (pitch + 2) * 4;
     const size_t lds = work > join ? work : join;      // (at most 35.8 KiB)
     const int64_t streams = (int64_t)a.rows * a.splits;
     const dim3 grid((unsigned)(a.qtiles == 1 ? streams : (streams + 7) / 8 * 8 * a.qtiles)), block(p.waves * 64);
