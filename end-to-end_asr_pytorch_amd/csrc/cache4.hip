@@ -257,8 +257,11 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
 // The weights go through LDS (16 bytes per token: all digits of all queries) into the A operand of the PV product - ds_read_b64_tr_b8 turns
 // them into rows (query, digit) - whose B operand, 16 tokens of one channel per lane, is what ds_read_b64_tr_b4 makes of the tile's
 // row-major codes.
-// The running reference m of a query is renewed only when a score passes it by 2^32 (weights are f32 and scaled per tile: nothing needs
-// them below 1), so a tile costs one reduction across the wave per query, the largest weight's, and four queries share its steps.
+// The running reference m of a query is renewed only when a score passes it by LAG (weights are f32 and scaled per tile: nothing needs them
+// below 1), so a tile costs one reduction across the wave per query, the largest weight's, and four queries share its steps.  Sums of weights
+// times values grow to 2^LAG times what the values themselves add up to, and have to stay below f32's 2^128: with LAG 8 that leaves 2^119
+// for the values of a row (|mid| + 8 scale) and a bit to spare.  LAG 32 takes 24 bits of that range and is no faster where the (base-2)
+// scores have a standard deviation of 1.4 (18 sizes and types within 1 %); at 5.8 it gains up to 2 % with 256 queries, nothing with few.
 // The next tile's loads are issued before the present one is worked on, the first tile's before the query is.
 //
 // What bounds it: HBM for long rows (72 bytes a token and head; 4 rows x 4 heads of 100003 slots, 16 splits: 19.5 us = 4.4 TB/s, + 3.9 us for
@@ -285,6 +288,7 @@ constexpr int PART = 66;      // floats of a partial result: 64 outputs (not div
 constexpr int MAX_NQ = 4, MAX_WAVES = 8, DENSE_ROW = 68;
 constexpr int TILE_V = 64 * 32, WAVE_LDS = TILE_V + 64 * 16;      // LDS bytes of a wave: a tile's codes of V; 16 bytes a token behind them
 constexpr float NO_REF = -3.4028234663852886e38f;
+constexpr float LAG = 8.f;      // log2
 
 // position of element k of 16 in the byte order that unpacking leaves: low nibbles of the first word, its high ones, then the second word's
 __device__ __forceinline__ int unpack_pos(int k) { return (k & 8) + (k & 1) * 4 + ((k >> 1) & 3); }
@@ -508,7 +512,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
             e[q] = __builtin_fmaf(s[q], unit[q], -m[q]);
             top = fmaxf(top, e[q]);
         }
-        if (__builtin_amdgcn_ballot_w64(top > 32.f)) {
+        if (__builtin_amdgcn_ballot_w64(top > LAG)) {
             const float big = NQ == 1 ? wave_all<MaxF>(s[0]) : wave_four<MaxF>(s[0], s[NQ > 1 ? 1 : 0], s[NQ > 2 ? 2 : 0], s[NQ > 3 ? 3 : 0]);      // of query c
             float f = 1.f;
 #pragma unroll
@@ -537,7 +541,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
             w[q] = p * (seen ? vsc : 0.f);
         }
         const float most = NQ == 1 ? wave_all<MaxPos>(w[0]) : wave_four<MaxPos>(w[0], w[1], w[2], w[3]);      // of query c
-        // (UNIT / most has to be finite: weights below 1e-30 of a reference that is within 2^32 of the largest probability count as 0)
+        // (UNIT / most has to be finite: weights below 1e-30 of a reference that is within 2^LAG of the largest probability count as 0)
         const float inv = most > 1e-30f ? D::UNIT * __builtin_amdgcn_rcpf(most) : 0.f, wunit = most * (1.f / (16.f * D::UNIT));
 #pragma unroll
         for (int q = 0; q < NQ; ++q) {
@@ -667,7 +671,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_dense_kernel(attn4
                     }
                 }
             }
-            if (__builtin_amdgcn_ballot_w64(top > 32.f)) {
+            if (__builtin_amdgcn_ballot_w64(top > LAG)) {
                 float big = s[0][0];
 #pragma unroll
                 for (int x = 1; x < 16; ++x) big = __builtin_elementwise_maximum(big, s[x >> 2][x & 3]);

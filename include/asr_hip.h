@@ -662,7 +662,8 @@ int asr_beam_advance(void* stream, int32_t* state, int32_t* k_len, int N, const 
  *   [N, h, Lq] (base 2) or NULL.  Slot j of row n is visible iff j < k_len[n] (int32 [N], cut to [0, T]; NULL: T) and, with `causal`, j <=
  *   k_len[n] - Lq + i for query i: the Lq queries are the last tokens of the row.  A query that sees nothing gets zeros and lse = -inf.
  *   Masked slots may hold anything.  Queries whose largest element is under 2^-100, and value scales times probability under 1e-30, count as
- *   0.  workspace: asr_cache4_attention_workspace_bytes() bytes (0: none needed), contents irrelevant, not shared
+ *   0.  Range, |mid| + 8 * scale of the visible slots: under 2^94 each in K (and finite scores), under 2^119 in V summed over a row; larger ones
+ *   may leave infinities or NaN in that row's result.  workspace: asr_cache4_attention_workspace_bytes() bytes (0: none needed), contents irrelevant, not shared
  *   by two launches that may run concurrently. */
 int asr_cache4_put(void* stream, const void* x, int x_dtype, int64_t s_kv, int64_t s_n, int64_t s_head, int64_t s_tok, void* codes, void* meta,
                    const int32_t* pos, int pos_stride, const int32_t* n_new, int n_kv, int N, int h, int L, int Tmax);

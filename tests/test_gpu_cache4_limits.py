@@ -1,0 +1,70 @@
+"""The 4-bit K / V cache at the ends of what asr_hip.h states for it: keys, and values whose sums come near f32's largest.  Expected
+values are 64-bit arithmetic on the stored codes."""
+import math
+
+import pytest
+import torch
+
+from asr_amd import ops
+from test_gpu_cache4 import rand_cache, reference
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+
+
+def check_rows(q, kc, vc, rows, causal=False):
+    """rows of the whole call against the 64-bit reference and its tolerance (test_gpu_cache4.reference)"""
+    T = kc.codes.shape[2]
+    got, lse = ops.cache4_attention(q, kc, vc, causal=causal, need_lse=True)
+    for n in rows:
+        one = lambda c: ops.Cache4(c.codes[n:n + 1].contiguous(), c.meta[n:n + 1].contiguous())  # noqa: E731
+        want, wl, tol, lt = reference(q[n:n + 1], one(kc), one(vc), [T], causal, q.dtype)
+        d = (got[n:n + 1].double().cpu() - want).abs()
+        assert bool((d <= tol).all()), "row %d: %s" % (n, "not finite" if not bool(d.isfinite().all()) else "worst %.3g of its tolerance" % float((d / tol).max()))
+        assert bool(((lse[n:n + 1].double().cpu() - wl).abs() <= lt).all())
+
+
+# one wave's second tile scores 2^30 times its first's: the first kernel, the same with split keys, the dense kernel
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("N,h,h_kv,Lq,T", [(2, 2, 2, 1, 1300), (1, 4, 1, 1, 1300), (1, 1, 1, 1, 5000), (100, 4, 4, 12, 600)])
+def test_large_values_behind_rising_scores(N, h, h_kv, Lq, T, causal, dtype):
+    """values around 2^100 - their sum over a row below 2^119 - where the scores rise by 30 half way along the row"""
+    g = torch.Generator().manual_seed(T + h)
+    c = rand_cache(g, 2, N, h_kv, T)
+    q = torch.zeros(N, h, Lq, 64, device=DEV, dtype=dtype)
+    q[..., 0] = 1.0
+    c.codes[0, ..., 0] = (c.codes[0, ..., 0] & 0xF0) | 1                     # the first channel's code is 1, the mid 0: score = scale
+    c.meta[0, ..., 1] = 0
+    rise = torch.where(torch.arange(T) < T // 2, 0.0, 30.0) + torch.rand(N, h_kv, T, generator=g)
+    c.meta[0, ..., 0] = rise.to(DEV)
+    big = torch.rand(2, N, h_kv, T, generator=g) + 0.5
+    c.meta[1, ..., 0] = (big[0] * 2.0 ** 98).to(DEV)
+    c.meta[1, ..., 1] = (torch.randn(N, h_kv, T, generator=g) * 2.0 ** 101).to(DEV)
+    total = (c.meta[1].double()[..., 1].abs() + 8 * c.meta[1].double()[..., 0]).sum(-1).max()
+    assert float(total) < 2.0 ** 119
+    check_rows(q, c[0], c[1], sorted({0, N - 1}), causal)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N,Lq,T", [(2, 2, 300), (100, 12, 150)])
+def test_large_keys(N, Lq, T, dtype):
+    """keys up to 2^94 beside queries small enough for scores of order one"""
+    g = torch.Generator().manual_seed(T)
+    c = rand_cache(g, 2, N, 4, T)
+    c.meta[0, ..., 0] = (torch.rand(N, 4, T, generator=g) * 2.0 ** 88).to(DEV)
+    c.meta[0, ..., 1] = (torch.randn(N, 4, T, generator=g).clamp(-3, 3) * 2.0 ** 91).to(DEV)
+    assert float((c.meta[0].double()[..., 1].abs() + 8 * c.meta[0].double()[..., 0]).max()) < 2.0 ** 94
+    q = (torch.randn(N, 4, Lq, 64, generator=g) * 2.0 ** -93).to(dtype).to(DEV)
+    check_rows(q, c[0], c[1], sorted({0, N - 1}))
+
+
+def test_finite_sums_stay_finite_with_many_slots():
+    """20 000 slots whose values add up to just under 2^119, equal scores: the mean comes out"""
+    T = 20000
+    c = ops.Cache4.empty(2, 1, 1, T, DEV)
+    v = 2.0 ** 104
+    c.meta[1, ..., 1] = v
+    got, _ = ops.cache4_attention(torch.zeros(1, 1, 1, 64, device=DEV), c[0], c[1])
+    assert T * v < 2.0 ** 119 and math.isfinite(float(got[0, 0, 0]))
+    assert bool(((got / v - 1).abs() <= 40 * 2.0 ** -24).all())
