@@ -86,11 +86,12 @@ template <typename T> __device__ __forceinline__ u32x2 quantise16(const float (&
     lo = __builtin_elementwise_minimum(lo, dpp_f<0x4E>(lo));
     hi = __builtin_elementwise_maximum(hi, dpp_f<0x4E>(hi));
     const float span = hi - lo;
-    const bool fine = span < INFINITY;
-    const float sc = span < 0x1p-100f || !fine ? 0.f : (float)(bf16_t)(span * (1.f / 15.f));      // (the format: a product, not a quotient)
+    const bool finite = span < INFINITY;
+    const float sc = span < 0x1p-100f || !finite ? 0.f : (float)(bf16_t)(span * (1.f / 15.f));      // (the format: a product, not a quotient)
     const float mid = (float)(bf16_t)(lo + 8.f * sc);
+    const bool fine = finite && fabsf(mid) < INFINITY;      // (a middle that rounds past bf16's largest is no middle)
     meta = fine ? bf16_bits(sc) | (bf16_bits(mid) << 16) : 0x7fc07fc0u;
-    if (sc == 0.f) return u32x2{0u, 0u};
+    if (sc == 0.f || !fine) return u32x2{0u, 0u};
     const float rs = __builtin_amdgcn_rcpf(sc);
     constexpr float MAGIC = 12582912.f + 8.f;      // 1.5 * 2^23: adding it rounds to the nearest integer, ties to even, and leaves code + 8 in the low bits
     float y[16], near = 0.f;

@@ -647,8 +647,9 @@ int asr_beam_advance(void* stream, int32_t* state, int32_t* k_len, int N, const 
  * Both contiguous; codes start on 16 bytes, meta on 4.  4.5 bits a value.  Quantising (asr_cache4_put), per slot:
  *   span = max - min;  scale = bf16(span * (1/15)), 0 where span < 2^-100;  mid = bf16(min + 8 * scale);  all in f32, 1/15 rounded to it
  *   code = (x - mid) / scale rounded to the nearest integer, ties to even - decided exactly, not from a rounded quotient -, cut to [-8, 7]
- *   (0 where scale is 0: a constant slot reads back as bf16 of its value).  A slot with a NaN or an infinity, or whose span overflows f32,
- *   gets scale = mid = NaN and reads back as NaN; where it is masked it is never looked at.
+ *   (0 where scale is 0: a constant slot reads back as bf16 of its value).  A slot with a NaN or an infinity, whose span overflows f32 or whose
+ *   mid overflows bf16 (values above 3.39e38) gets scale = mid = NaN, codes 0, and reads back as NaN; where it is masked it is never looked
+ *   at.  A value is held to half a step, so the largest of a row may read back as an infinity where half a step more is one.
  * asr_cache4_put:  x (f32 | bf16) [n_kv, N, h, L, 64] by element strides s_kv / s_n / s_head / s_tok, the 64 values of a row adjacent, rows on
  *   16 bytes (strides multiples of 8 in bf16, 4 in f32): token i < n_new[n] goes to slot pos[n * pos_stride] + i.  pos NULL: 0; pos_stride 0:
  *   one position for all rows (&state[0] of the decoding step), 1: int32 [N].  n_new NULL: all L.  A slot outside [0, Tmax) is not written, and

@@ -1,15 +1,17 @@
-"""The 4-bit K / V cache at the ends of what asr_hip.h states for it: keys, and values whose sums come near f32's largest.  Expected
-values are 64-bit arithmetic on the stored codes."""
+"""The 4-bit K / V cache at the ends of what asr_hip.h states for it: keys, values whose sums come near f32's largest, and
+rows near bf16's largest.  Expected values are 64-bit arithmetic on the stored codes, or equality."""
 import math
 
 import pytest
 import torch
 
 from asr_amd import ops
-from test_gpu_cache4 import rand_cache, reference
+from test_gpu_cache4 import rand_cache, reference, same, values
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
+F32_MAX = torch.finfo(torch.float32).max
+BF16_MAX = torch.finfo(torch.bfloat16).max
 
 
 def check_rows(q, kc, vc, rows, causal=False):
@@ -57,6 +59,29 @@ def test_large_keys(N, Lq, T, dtype):
     assert float((c.meta[0].double()[..., 1].abs() + 8 * c.meta[0].double()[..., 0]).max()) < 2.0 ** 94
     q = (torch.randn(N, 4, Lq, 64, generator=g) * 2.0 ** -93).to(dtype).to(DEV)
     check_rows(q, c[0], c[1], sorted({0, N - 1}))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_near_the_largest_value(dtype):
+    """a row is finite (code, scale and middle) or NaN, never a middle of infinity: constants and narrow rows on both sides of bf16's largest"""
+    fine = [torch.full((64,), BF16_MAX), torch.full((64,), -BF16_MAX), torch.linspace(0.0, BF16_MAX, 64), torch.linspace(-BF16_MAX, 0.0, 64),
+            torch.linspace(3.0e38, 3.35e38, 64)]
+    over = []
+    if dtype == torch.float32:      # (bf16 has no finite value above its largest; its half step ends at 3.396e38)
+        over = [torch.full((64,), F32_MAX), torch.full((64,), -F32_MAX), torch.linspace(3.397e38, 3.402e38, 64), -torch.linspace(3.397e38, 3.402e38, 64)]
+    x = torch.stack(fine + over).to(dtype).to(DEV)[None, None]
+    c = ops.Cache4.empty(None, 1, 1, x.shape[2], DEV)
+    ops.cache4_put(c, x)
+    n = len(fine)
+    assert bool(c.meta[0, 0, :n].isfinite().all())
+    assert bool(c.meta[0, 0, n:].isnan().all()) and int(c.codes[0, 0, n:].max() if over else 0) == 0
+    got = ops.cache4_get(c, dtype=torch.float32)
+    assert same(got, values(c)) and bool(got[0, 0, n:].isnan().all())
+    assert torch.equal(got[0, 0, :2], torch.tensor([[BF16_MAX], [-BF16_MAX]], device=DEV).expand(2, 64))
+    # within the middle's half step (2^-9 of it) and half a code's step (with the middle's own rounding in it) of the value, both bf16
+    d = (got[0, 0, 2:n].double() - x[0, 0, 2:n].double()).abs()
+    scale, mid = c.meta[0, 0, 2:n].double().unbind(-1)
+    assert bool((d <= (scale / 2 + mid.abs() * 2.0 ** -8)[:, None]).all())
 
 
 def test_finite_sums_stay_finite_with_many_slots():
