@@ -208,15 +208,15 @@ __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, st
 // ---- re-gathering by parent ------------------------------------------------------------------------------------------------------------
 // A group is one (kv, utterance, head).  A block takes 256 pieces of its positions - 16-byte halves of the codes, or meta words - and a thread
 // its piece for all the beam's rows: it reads every source row's before it writes any, so source and destination may be the same cache.  The
-// parents are the same for a whole block: scalar loads, row addresses in scalar registers (with them in vector registers: 236 VGPRs, 70 us).
+// parents are the same for a whole block: lane r of a wave reads row r's, row addresses are scalar (with them in vector registers: 236 VGPRs, 70 us).
 // Measured: 12 x 8 utterances x 8 beams x 4 heads x 777 positions into another cache 38.5 us = 4.5 TB/s; a step of 32 x 5 beams, 51 positions 7 us.
-template <typename V, int BEAM> __device__ __forceinline__ void regather(const V* src, V* dst, const int64_t* parent, int64_t first, int64_t row, int beam, unsigned u,
+template <typename V, int BEAM> __device__ __forceinline__ void regather(const V* src, V* dst, int mine, int64_t row, int beam, unsigned u,
                                                                          bool in_place) {
     V v[BEAM];
     int from[BEAM];
 #pragma unroll
     for (int r = 0; r < BEAM; ++r) {
-        from[r] = r < beam ? clampi((int)(parent[r] - first), 0, beam - 1) : r;
+        from[r] = __builtin_amdgcn_readlane(mine, r);
         if (r < beam && !(in_place && from[r] == r)) v[r] = (src + (int64_t)from[r] * row)[u];
     }
 #pragma unroll
@@ -236,10 +236,14 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
     const bool is_meta = chunk >= chunks_codes;
     if (is_meta) chunk -= chunks_codes;
     const unsigned u = chunk * 256u + threadIdx.x;
-    if (u >= (unsigned)(is_meta ? n : 2 * n)) return;
-    parent += (int64_t)b * beam;
-    if (is_meta) regather<uint32_t, BEAM>(meta + row0, out_meta + row0, parent, (int64_t)b * beam, (int64_t)h * Tmax, beam, u, in_place);
-    else regather<u32x4, BEAM>(codes + row0 * 2, out_codes + row0 * 2, parent, (int64_t)b * beam, (int64_t)h * Tmax * 2, beam, u, in_place);
+    const unsigned live = is_meta ? n : 2 * n;
+    if ((u & ~63u) >= live) return;      // (whole waves: in the others all lanes are there for the parents)
+    // lane r: the source row of row r within the utterance.  Compared as 64 bits: an id far outside must not come back modulo 2^32
+    const int64_t first = (int64_t)b * beam, id = parent[first + min((int)threadIdx.x & 63, beam - 1)];
+    const int mine = id < first ? 0 : id < first + beam ? (int)(id - first) : beam - 1;
+    if (u >= live) return;
+    if (is_meta) regather<uint32_t, BEAM>(meta + row0, out_meta + row0, mine, (int64_t)h * Tmax, beam, u, in_place);
+    else regather<u32x4, BEAM>(codes + row0 * 2, out_codes + row0 * 2, mine, (int64_t)h * Tmax * 2, beam, u, in_place);
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------------------------

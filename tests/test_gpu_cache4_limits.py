@@ -1,12 +1,12 @@
-"""The 4-bit K / V cache at the ends of what asr_hip.h states for it: keys, values whose sums come near f32's largest, and
-rows near bf16's largest.  Expected values are 64-bit arithmetic on the stored codes, or equality."""
+"""The 4-bit K / V cache at the ends of what asr_hip.h states for it: keys, values whose sums come near f32's largest,
+rows near bf16's largest, parents outside their utterance.  Expected values are 64-bit arithmetic on the stored codes, or equality."""
 import math
 
 import pytest
 import torch
 
 from asr_amd import ops
-from test_gpu_cache4 import rand_cache, reference, same, values
+from test_gpu_cache4 import i32, rand_cache, reference, same, values
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -82,6 +82,24 @@ def test_rows_near_the_largest_value(dtype):
     d = (got[0, 0, 2:n].double() - x[0, 0, 2:n].double()).abs()
     scale, mid = c.meta[0, 0, 2:n].double().unbind(-1)
     assert bool((d <= (scale / 2 + mid.abs() * 2.0 ** -8)[:, None]).all())
+
+
+@pytest.mark.parametrize("in_place", [True, False])
+def test_parents_outside_their_utterance(in_place):
+    """cut to the nearest row of the utterance, however far outside: not modulo 2^32"""
+    beam, B, T = 8, 3, 20
+    g = torch.Generator().manual_seed(1)
+    c = rand_cache(g, 2, B * beam, 2, T)
+    parent, rows = [], []
+    for b in range(B):
+        first = b * beam
+        parent += [first - 1, first + beam, first + 2 ** 32, first - 2 ** 32 + 3, first + 2 ** 31, first - 2 ** 40, -2 ** 63, 2 ** 63 - 1]
+        rows += [first, first + beam - 1, first + beam - 1, first, first + beam - 1, first, first, first + beam - 1]
+    before = ops.Cache4(c.codes.clone(), c.meta.clone())
+    out = None if in_place else rand_cache(g, 2, B * beam, 2, T)
+    ops.cache4_reorder(c, torch.tensor(parent, dtype=torch.int64, device=DEV), i32(T - 1, -1), beam, out=out)
+    got = c if in_place else out
+    assert torch.equal(got.codes, before.codes[:, rows]) and torch.equal(got.meta, before.meta[:, rows])
 
 
 def test_finite_sums_stay_finite_with_many_slots():
