@@ -7,6 +7,7 @@ no arithmetic on the product path is done by torch ops.  There is no CPU fallbac
 import atexit
 import ctypes
 import functools
+import operator
 import weakref
 import os
 import threading
@@ -1412,6 +1413,8 @@ class Cache4:
     def __getitem__(self, i):
         if not self.stack:
             raise IndexError("Cache4: one cache, not a stack")
+        if type(i) not in (int, slice):
+            i = operator.index(i)      # (TypeError for lists and masks: they would copy)
         return Cache4(self.codes[i], self.meta[i])
 
     def __len__(self):

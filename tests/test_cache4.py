@@ -1,6 +1,7 @@
 """The 4-bit K / V cache's entry points without a GPU: what they refuse, and the size query."""
 import ctypes
 
+import numpy as np
 import pytest
 import torch
 
@@ -21,6 +22,20 @@ def test_cache4_shapes_and_views():
     with pytest.raises(IndexError):
         c[0][0]
     assert c[2:4].shape == (2, 3, 4, 8) and c[2:4].codes.data_ptr() == c[2].codes.data_ptr()
+
+
+@pytest.mark.parametrize("index", [[0, 2], torch.tensor([0, 2]), torch.tensor([True] * 2 + [False] * 4), (0, 1), None, ...])
+def test_cache4_indices_that_would_copy_are_refused(index):
+    """a list or a mask would make another cache: what is put there would not be in this one"""
+    with pytest.raises(TypeError):
+        ops.Cache4.empty(6, 3, 4, 8, "cpu")[index]
+
+
+def test_cache4_whole_number_indices():
+    c = ops.Cache4.empty(6, 3, 4, 8, "cpu")
+    for i in (-1, torch.tensor(5), np.int64(5)):
+        assert c[i].codes.data_ptr() == c.codes[5].data_ptr()
+    assert len([k for k in c]) == 6
 
 
 @pytest.mark.parametrize("codes,meta,err", [
