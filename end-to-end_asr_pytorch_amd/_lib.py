@@ -178,35 +178,59 @@ def existing_sources():
     return [s for s in SOURCES if os.path.exists(os.path.join(CSRC, s))]
 
 
+def _record(path, text=None):
+    """the command that made `path`, kept beside the objects: read it, or (text) note it; '' forgets it"""
+    r = os.path.join(CSRC, "build", os.path.basename(path) + ".cmd")
+    if text is None:
+        return open(r).read() if os.path.exists(r) else None
+    if text:
+        with open(r, "w") as f:
+            f.write(text)
+    elif os.path.exists(r):
+        os.unlink(r)
+
+
 def build_library(force=False, verbose=False):
-    """hipcc --offload-arch=gfx950 -shared -fPIC csrc/*.hip -o csrc/libasr_hip.so (rebuilt only when stale)."""
+    """hipcc --offload-arch=gfx950 -shared -fPIC csrc/*.hip -o csrc/libasr_hip.so (rebuilt only when stale: older than a source, or made by
+    another command line - an object without its record counts as that)."""
     srcs = [os.path.join(CSRC, s) for s in existing_sources()]
     incs = sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(".inc"))     # generated instruction streams (tools/gen_attn_*.py)
     deps = srcs + incs + [os.path.join(CSRC, "asr_common.h"), HEADER]
-    if not force and os.path.exists(LIB_PATH) and all(os.path.getmtime(LIB_PATH) >= os.path.getmtime(d) for d in deps):
+    extra = os.environ.get("ASR_AMD_EXTRA_HIPCC_FLAGS", "").split()      # (diagnostic builds: -DHEADS_ABLATE, -DFFN_STAMP ...)
+    cmds = [[hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_F32 + EXTRA_FLAGS.get(os.path.basename(s), []) + extra for s in srcs]
+    records = [" ".join(c) for c in cmds]      # (without the paths: a tree may be copied)
+    whole = "\n".join(records)
+    if not force and os.path.exists(LIB_PATH) and _record(LIB_PATH) == whole and all(os.path.getmtime(LIB_PATH) >= os.path.getmtime(d) for d in deps):
         return LIB_PATH
     objs = []
     procs = []
     os.makedirs(os.path.join(CSRC, "build"), exist_ok=True)
-    for s in srcs:
+    _record(LIB_PATH, "")
+    for s, cmd, record in zip(srcs, cmds, records):
         o = os.path.join(CSRC, "build", os.path.basename(s) + ".o")
         objs.append(o)
-        if not force and os.path.exists(o) and all(
+        if not force and os.path.exists(o) and _record(o) == record and all(
                 os.path.getmtime(o) >= os.path.getmtime(d) for d in [s, deps[-2], deps[-1]] + incs):
             continue
-        cmd = [hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_F32 + EXTRA_FLAGS.get(os.path.basename(s), []) + \
-            os.environ.get("ASR_AMD_EXTRA_HIPCC_FLAGS", "").split() + ["-c", s, "-o", o]      # (diagnostic builds: -DHEADS_ABLATE, -DFFN_STAMP ...)
+        _record(o, "")      # (a compiler that fails may have written something)
+        cmd = cmd + ["-c", s, "-o", o]
         if verbose:
             print(" ".join(cmd))
-        procs.append((cmd, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
-    for cmd, p in procs:
+        procs.append((cmd, o, record, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))
+    failed = None
+    for cmd, o, record, p in procs:
         out, _ = p.communicate()
-        if p.returncode != 0:
-            raise RuntimeError("hipcc failed: %s\n%s" % (" ".join(cmd), out.decode(errors="replace")))
+        if p.returncode == 0:
+            _record(o, record)
+        elif failed is None:
+            failed = "hipcc failed: %s\n%s" % (" ".join(cmd), out.decode(errors="replace"))
+    if failed is not None:
+        raise RuntimeError(failed)
     cmd = [hipcc_path(), "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB_PATH] + objs
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     if r.returncode != 0:
         raise RuntimeError("link failed: %s\n%s" % (" ".join(cmd), r.stdout.decode(errors="replace")))
+    _record(LIB_PATH, whole)
     return LIB_PATH
 
 
