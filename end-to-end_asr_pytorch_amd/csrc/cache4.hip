@@ -287,7 +287,7 @@ struct attn4_t {
     const u32x4* kc; const uint32_t* km; const u32x4* vc; const uint32_t* vm;
     void* ctx; float* lse; float* part;
     const int32_t* k_len;
-    int N, h, h_kv, Lq, T, splits, qtiles, per_tile, rows, waves;
+    int h, h_kv, Lq, T, splits, qtiles, per_tile, rows, waves;
 };
 constexpr int PART = 66;      // floats of a partial result: 64 outputs (not divided), reference, sum
 constexpr int MAX_NQ = 4, MAX_WAVES = 8, DENSE_ROW = 68;
@@ -374,7 +374,7 @@ __device__ __forceinline__ void load_tile(tile4_t& t, const u32x4* kc, const u32
 // ---- what the two attention kernels share -----------------------------------------------------------------------------------------------
 struct work4_t { int row, split, n, hk, group, q0, nq; int64_t base; };
 // block -> (row, query tile, split): the query tiles of one stream of keys follow each other at a distance of 8 blocks (one XCD's L2)
-__device__ __forceinline__ bool work_of(const attn4_t& a, int width, work4_t& b) {
+__device__ __forceinline__ bool work_of(const attn4_t& a, work4_t& b) {
     int stream = blockIdx.x, qt = 0;
     if (a.qtiles > 1) {
         const int per8 = 8 * a.qtiles, oct = stream / per8, rest = stream - oct * per8;
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = a.waves, n16 = lane & 15, c = lane >> 4;
     work4_t b;
-    if (!work_of(a, NQ, b)) return;
+    if (!work_of(a, b)) return;
     const u32x4* kc = a.kc + b.base * 2;
     const u32x4* vc = a.vc + b.base * 2;
     const uint32_t* km = a.km + b.base;
@@ -601,7 +601,7 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_dense_kernel(attn4
     extern __shared__ __align__(16) unsigned char lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), W = a.waves, n16 = lane & 15, c = lane >> 4;
     work4_t b;
-    if (!work_of(a, DENSE_NQ, b)) return;
+    if (!work_of(a, b)) return;
     const u32x2* kc = reinterpret_cast<const u32x2*>(a.kc + b.base * 2);
     const u32x4* vc = a.vc + b.base * 2;
     const uint32_t* km = a.km + b.base;
@@ -829,7 +829,8 @@ plan_t attn_plan(int rows, int Q, int T) {
 template <typename T, int ND> int attn_launch(hipStream_t s, const attn4_t& a, const plan_t& p, bool causal) {
     const int width = p.dense ? DENSE_NQ : p.nq, pitch = p.dense ? DENSE_ROW : 64;
     const size_t work = (size_t)p.waves * WAVE_LDS + width * (ND * 64 + 8), join = (size_t)p.waves * width * (pitch + 2) * 4;
-    const size_t lds = work > join ? work : join;      // (at most 35.8 KiB)
+    const size_t lds = work > join ? work : join;
+    static_assert(MAX_WAVES * DENSE_NQ * (DENSE_ROW + 2) * 4 <= 40 * 1024 && MAX_WAVES * WAVE_LDS + DENSE_NQ * (ND * 64 + 8) <= 40 * 1024, "a quarter of a CU's 160 KiB");
     const int64_t streams = (int64_t)a.rows * a.splits;
     const dim3 grid((unsigned)(a.qtiles == 1 ? streams : (streams + 7) / 8 * 8 * a.qtiles)), block(p.waves * 64);
 #define ASR_C4(...)                                                                                     \
@@ -961,7 +962,7 @@ extern "C" int asr_cache4_attention(void* stream, const void* q, int dtype, int6
     ASR_REQUIRE(need == 0 || (workspace && workspace_bytes >= need && asr_aligned(workspace, 4)), ASR_ERR_ARG, "cache4_attention: workspace of %lld bytes needed, %lld given",
                 (long long)need, (long long)(workspace ? workspace_bytes : 0));
     attn4_t a{q, s_n, s_head, s_tok, static_cast<const u32x4*>(k_codes), static_cast<const uint32_t*>(k_meta), static_cast<const u32x4*>(v_codes),
-              static_cast<const uint32_t*>(v_meta), ctx, lse, static_cast<float*>(workspace), k_len, N, h, h_kv, Lq, T, p.splits, p.qtiles, p.nq,
+              static_cast<const uint32_t*>(v_meta), ctx, lse, static_cast<float*>(workspace), k_len, h, h_kv, Lq, T, p.splits, p.qtiles, p.nq,
               N * h_kv, p.waves};
     hipStream_t s = static_cast<hipStream_t>(stream);
     return dtype == ASR_BF16 ? attn_launch<bf16_t, 2>(s, a, p, causal != 0) : attn_launch<float, 3>(s, a, p, causal != 0);
