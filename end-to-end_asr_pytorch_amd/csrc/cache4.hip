@@ -61,9 +61,10 @@ __device__ __forceinline__ float quotient(float d, float s, float rs) {
     return __builtin_fmaf(__builtin_fmaf(-y, s, d), rs, y);
 }
 
-// Quantising reads 128 (bf16) or 256 bytes a row and writes 36: HBM, with the VALU next to it (11 instructions a value).  4 lanes a row share the
-// row's own arithmetic (8 lanes: 3 instructions a value more); the next row's loads are in flight while this one is worked on.  Measured:
-// 12 x 32 x 4 rows of 1000 tokens in bf16 53 us = 4.7 TB/s (a copy of 1 GiB moves 5.2 here); 47 us = 4.0 with rows of 500 to 1000 tokens.
+// Quantising reads 128 (bf16) or 256 bytes a row and writes 36: HBM, with the VALU next to it (11 instructions a value, 27 us of issue at 2.4 GHz
+// for the 1.15 M rows below).  4 lanes a row share the row's own arithmetic (8 lanes: 3 instructions a value more); the next row's loads are
+// in flight while this one is worked on.  Measured: 12 x 32 x 4 rows of 1000 tokens in bf16 54.5 us = 4.6 TB/s (a copy of 1 GiB moves 5.15 here);
+// rows of 500 to 1000 tokens 60 us = 3.2 TB/s behind a launch whose 197 MB of results are still on their way to memory (51 at best).
 //
 // The codes of 16 values of a row whose 64 values lie in 4 neighbouring lanes: -> the two 32-bit words of nibbles, and the row's (scale, mid).
 // Every decision is that of (x - mid) / scale computed exactly.  The corrected quotient settles it unless the subtraction was rounded and
@@ -182,7 +183,7 @@ __global__ __launch_bounds__(256) void cache4_put_kernel(const T* __restrict__ x
 }
 
 // Reading back: 36 bytes in, 128 or 256 out.  8 lanes a row, 16 bytes (bf16) of output each: whole cache lines per store.  Measured: 12 x 32 x 4
-// rows of 1000 tokens to bf16 44 us = 5.7 TB/s.
+// rows of 1000 tokens to bf16 42.8 us = 5.9 TB/s.
 template <typename T, bool ONE_ROW>
 __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, strides_t st, const uint32_t* __restrict__ codes,
                                                          const uint32_t* __restrict__ meta, slots_t s) {
@@ -209,7 +210,8 @@ __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, st
 // A group is one (kv, utterance, head).  A block takes 256 pieces of its positions - 16-byte halves of the codes, or meta words - and a thread
 // its piece for all the beam's rows: it reads every source row's before it writes any, so source and destination may be the same cache.  The
 // parents are the same for a whole block: lane r of a wave reads row r's, row addresses are scalar (with them in vector registers: 236 VGPRs, 70 us).
-// Measured: 12 x 8 utterances x 8 beams x 4 heads x 777 positions into another cache 38.5 us = 4.5 TB/s; a step of 32 x 5 beams, 51 positions 7 us.
+// Measured: 12 x 8 utterances x 8 beams x 4 heads x 777 positions into another cache 44 us = 3.9 TB/s (40 at best), 29.6 where the Infinity Cache
+// holds both, 26.5 there in place; a step of 32 x 5 beams, 51 positions 8.1 us, in place 7.3.
 template <typename V, int BEAM> __device__ __forceinline__ void regather(const V* src, V* dst, int mine, int64_t row, int beam, unsigned u,
                                                                          bool in_place) {
     V v[BEAM];
@@ -269,9 +271,9 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
 // scores have a standard deviation of 1.4 (18 sizes and types within 1 %); at 5.8 it gains up to 2 % with 256 queries, nothing with few.
 // The next tile's loads are issued before the present one is worked on, the first tile's before the query is.
 //
-// What bounds it: HBM for long rows (72 bytes a token and head; 4 rows x 4 heads of 100003 slots, 16 splits: 19.5 us = 4.4 TB/s, + 3.9 us for
-// the join), launch and one chain of loads for a decoding step (32 x 4 rows of 1000 slots: 5.3 us with one query, 7.0 with five), the VALU
-// and the chain of a tile for many queries (the dense kernel below).
+// What bounds it: HBM for long rows (72 bytes a token and head; 4 rows x 4 heads of up to 100003 slots, 16 splits: 20.5 us = 4.6 TB/s, + 3.9 us for
+// the join), launch and one chain of loads for a decoding step (32 x 4 rows of 1000 slots: 5.3 us a replayed call with one query, 6.5 with
+// five), the VALU and the chain of a tile for many queries (the dense kernel below).
 template <int ND> struct Digits {
     static constexpr float UNIT = ND == 2 ? 127.f * 256.f : 127.f * 65536.f;      // the integer that the largest element becomes
     static constexpr int BIAS = ND == 2 ? 0x80 : 0x8080;                          // u + BIAS, its lower bytes' sign bits inverted: the digits, lowest first
@@ -592,8 +594,9 @@ __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_kernel(attn4_t a) 
 // Many queries: the same products turned round.  K is the A operand (16 tokens a row, 8 bytes of codes a lane), 16 queries the columns, so a lane
 // holds the scores of ONE query for 16 of the tile's 64 tokens - statistics, masks and scales are per lane - and those 16 weights are, as they
 // stand, the lane's share of the PV product's B operand: no LDS between the two products.  V is the A operand (ds_read_b64_tr_b4, its rows read
-// in the order in which the lane holds the tokens), the output [channel, query].  About 390 VALU instructions a tile for 16 queries where the
-// kernel above takes 200 for four; the tokens' scales reach the lanes through LDS.
+// in the order in which the lane holds the tokens), the output [channel, query].  430 VALU instructions a tile for 16 queries (counted over rows of 313
+// tiles) where the kernel above takes 205 for four; the tokens' scales reach the lanes through LDS.  64 rows x 33 causal queries x up to 2011
+// slots: 12.7 us; VALU issue fills 6 us of it on the 192 CUs that have a block, the rest is the chain of a tile (QK, maximum, digits, PV).
 constexpr int DENSE_NQ = 16;
 template <typename T, int ND, bool CAUSAL>
 __global__ __launch_bounds__(MAX_WAVES * 64) void cache4_attn_dense_kernel(attn4_t a) {
@@ -794,17 +797,18 @@ __global__ __launch_bounds__(JOIN_WAVES * 64) void cache4_join_kernel(attn4_t a)
 
 // How a call is cut.  Times in us, bf16, graph replays, keys cold where they do not fit the caches.
 //   kernel            the dense one does half the work a query and has the longer chain a tile: from 9 queries a key head up, where there is work
-//                     for many waves - 12 tiles of four queries a SIMD, or four blocks a CU.  64 rows x 2011 slots: 33 queries 12.0 against 15.5, 128
-//                     queries 20.6 against 32.0, but 16 queries 12.3 against 8.7; 640 rows x 101 slots: 16 queries 11.0 against 12.7, 8 queries 9.0
-//                     against 8.0; 8 rows x 20000 slots: 64 queries 17.7 against 24.1, 16 queries 13.1 against 12.4
+//                     for many waves - 12 tiles of four queries a SIMD, or four blocks a CU.  64 rows x 2011 slots: 33 queries 12.3 against 16.5, 128
+//                     queries 20.3 against 33.1, but 16 queries 12.3 against 8.7; 640 rows x 101 slots: 16 queries 10.9 against 12.8, 8 queries 8.9
+//                     against 8.1; 8 rows x 20000 slots: 64 queries 18.3 against 26.4, 16 queries 12.4 either way
 //   queries a block   up to 4 (16 in the dense kernel), evenly: eight in the first kernel need 184 VGPRs instead of 106 and lose at every size (5
-//                     queries x 128 rows x 1000 slots 8.4 against 7.1)
-//   waves             one per tile of 64 slots up to 8; 4 where more blocks than CUs make a CU take two anyway (300 rows x 2000 slots 12.6 with 8,
-//                     11.6 with 4; 230 rows 8.8 and 9.3; 128 rows x 1000 slots 5.8 with 8, 5.9 with 4, 7.7 with 2).  The dense kernel's waves also
-//                     share the queries' digits: never fewer for few tiles (640 rows x 101 slots: 11.0 with 4, 12.4 with 2)
+//                     queries x 128 rows x 1000 slots 8.4 against 7.1; three a block 6.9, two 7.8)
+//   waves             one per tile of 64 slots up to 8; 4 where more blocks than CUs make a CU take two anyway (300 rows x 2000 slots 12.9 with 8,
+//                     11.8 with 4; 230 rows 9.3 and 9.3; 128 rows x 1000 slots 6.0 with 8, 6.1 with 4, 7.8 with 2).  The dense kernel's waves also
+//                     share the queries' digits: never fewer for few tiles (640 rows x 101 slots: 11.1 with 4, 12.7 with 2)
 //   splits            where a wave would walk more than 4 tiles and there are no more than 128 blocks: as many as fill 256 CUs with a block each,
-//                     two tiles a wave at least (16 rows x 100003 slots: 1 split 168, 16 splits 26.6, 32 splits 27.8; 4 rows: 32 splits 11.6, 20
-//                     13.4).  Below that the second launch costs more than it gives (20 rows x 777 slots 4.9 against 6.4).
+//                     two tiles a wave at least (16 rows x 100003 slots: 1 split 143, 16 splits 26.0, 32 splits 26.6; 4 rows: 32 splits 11.7, 20
+//                     13.5).  Below that the second launch costs more than it gives (20 rows x 777 slots 4.9 against 6.8; 130 rows x 6000 15.1
+//                     against 19.6).
 struct plan_t { int nq, qtiles, splits, waves; bool dense; };
 plan_t attn_plan(int rows, int Q, int T) {
     plan_t p;
@@ -867,6 +871,8 @@ int slots_plan(const char* name, int lanes, slots_t& s, int64_t& blocks, int n_k
     const int groups_log2 = lanes == 4 ? 6 : 5;      // rows of 64 values side by side in a block of 256 threads
     int lg = 0;
     while (lg < groups_log2 && (1 << lg) < L) ++lg;
+    // a group of lanes walks 4 rows: reading back 12 x 32 x 4 x 1000 rows 42.8 us (49.8 with 2, 43.9 with 8), put 54.6 (53.8, 55.7).  It costs the calls
+    // of few blocks a chain of loads: 2 x 7 x 4 x 333 f32 rows put 5.4 and read back 4.5 (3.9 and 3.9 with one row each)
     const int rb_log2 = groups_log2 - lg, iter = 4, chunks = (int)((L + ((int64_t)iter << lg) - 1) / ((int64_t)iter << lg));
     blocks = (rows + (1 << rb_log2) - 1) / (1 << rb_log2) * chunks;
     ASR_REQUIRE(blocks <= MAX_BLOCKS, ASR_ERR_UNSUPPORTED, "%s: too many rows", name);
