@@ -200,12 +200,14 @@ def build_library(force=False, verbose=False):
     cmds = [[hipcc_path(), "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC"] + NO_PACKED_F32 + EXTRA_FLAGS.get(os.path.basename(s), []) + extra for s in srcs]
     records = [" ".join(c) for c in cmds]      # (without the paths: a tree may be copied)
     whole = "\n".join(records)
-    if not force and os.path.exists(LIB_PATH) and _record(LIB_PATH) == whole and all(os.path.getmtime(LIB_PATH) >= os.path.getmtime(d) for d in deps):
+    own = os.path.dirname(os.path.abspath(LIB_PATH)) == os.path.abspath(CSRC)      # (another build for comparisons has flags of its own)
+    if not force and os.path.exists(LIB_PATH) and (not own or _record(LIB_PATH) == whole) and all(os.path.getmtime(LIB_PATH) >= os.path.getmtime(d) for d in deps):
         return LIB_PATH
     objs = []
     procs = []
     os.makedirs(os.path.join(CSRC, "build"), exist_ok=True)
-    _record(LIB_PATH, "")
+    if own:
+        _record(LIB_PATH, "")
     for s, cmd, record in zip(srcs, cmds, records):
         o = os.path.join(CSRC, "build", os.path.basename(s) + ".o")
         objs.append(o)
@@ -230,7 +232,8 @@ def build_library(force=False, verbose=False):
     r = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)
     if r.returncode != 0:
         raise RuntimeError("link failed: %s\n%s" % (" ".join(cmd), r.stdout.decode(errors="replace")))
-    _record(LIB_PATH, whole)
+    if own:
+        _record(LIB_PATH, whole)
     return LIB_PATH
 
 

@@ -74,3 +74,16 @@ def test_a_failed_compile_is_not_taken_for_done(tree):
         tree()
     (tree.tmp / "broken").unlink()
     assert tree() == (["a.hip"], True)      # (the compiler had written its output before it failed)
+
+
+def test_a_library_elsewhere_is_left_alone_while_it_is_newer(tree, monkeypatch, tmp_path):
+    """ASR_AMD_LIB names another build for comparisons: its flags are its own business, and this tree's record is not its"""
+    tree()
+    other = tmp_path / "lib.so"
+    other.write_text("another build")
+    monkeypatch.setattr(_lib, "LIB_PATH", str(other))
+    assert tree() == ([], False) and other.read_text() == "another build"
+    os.utime(other, (1, 1))
+    assert tree() == ([], True)                        # (older than the sources: linked anew, as ever)
+    monkeypatch.setattr(_lib, "LIB_PATH", str(tree.csrc / "lib.so"))
+    assert tree() == ([], False)
