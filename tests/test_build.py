@@ -79,7 +79,7 @@ def test_a_failed_compile_is_not_taken_for_done(tree):
 def test_a_library_elsewhere_is_left_alone_while_it_is_newer(tree, monkeypatch, tmp_path):
     """ASR_AMD_LIB names another build for comparisons: its flags are its own business, and this tree's record is not its"""
     tree()
-    other = tmp_path / "lib.so"
+    other = tmp_path / "other.so"
     other.write_text("another build")
     monkeypatch.setattr(_lib, "LIB_PATH", str(other))
     assert tree() == ([], False) and other.read_text() == "another build"
