@@ -211,14 +211,14 @@ __global__ __launch_bounds__(256) void cache4_get_kernel(T* __restrict__ out, st
 // its piece for all the beam's rows: it reads every source row's before it writes any, so source and destination may be the same cache.  The
 // parents are the same for a whole block: lane r of a wave reads row r's, row addresses are scalar (with them in vector registers: 236 VGPRs, 70 us).
 // Measured: 12 x 8 utterances x 8 beams x 4 heads x 777 positions into another cache 44 us = 3.9 TB/s (40 at best), 29.6 where the Infinity Cache
-// holds both, 26.5 there in place; a step of 32 x 5 beams, 51 positions 8.1 us, in place 7.3.
-template <typename V, int BEAM> __device__ __forceinline__ void regather(const V* src, V* dst, int mine, int64_t row, int beam, unsigned u,
+// holds both, 26.5 there in place; a step of 32 x 5 beams, 51 positions 8.2 us, in place 7.4.
+template <typename V, int BEAM> __device__ __forceinline__ void regather(const V* src, V* dst, unsigned parents, int64_t row, int beam, unsigned u,
                                                                          bool in_place) {
     V v[BEAM];
     int from[BEAM];
 #pragma unroll
     for (int r = 0; r < BEAM; ++r) {
-        from[r] = __builtin_amdgcn_readlane(mine, r);
+        from[r] = (parents >> (4 * r)) & 15;
         if (r < beam && !(in_place && from[r] == r)) v[r] = (src + (int64_t)from[r] * row)[u];
     }
 #pragma unroll
@@ -243,9 +243,12 @@ __global__ __launch_bounds__(256) void cache4_reorder_kernel(const u32x4* codes,
     // lane r: the source row of row r within the utterance.  Compared as 64 bits: an id far outside must not come back modulo 2^32
     const int64_t first = (int64_t)b * beam, id = parent[first + min((int)threadIdx.x & 63, beam - 1)];
     const int mine = id < first ? 0 : id < first + beam ? (int)(id - first) : beam - 1;
+    unsigned parents = 0;      // four bits a row.  (Read in front of the return: behind it lane r may be gone)
+#pragma unroll
+    for (int r = 0; r < BEAM; ++r) parents |= (unsigned)__builtin_amdgcn_readlane(mine, r) << (4 * r);
     if (u >= live) return;
-    if (is_meta) regather<uint32_t, BEAM>(meta + row0, out_meta + row0, mine, (int64_t)h * Tmax, beam, u, in_place);
-    else regather<u32x4, BEAM>(codes + row0 * 2, out_codes + row0 * 2, mine, (int64_t)h * Tmax * 2, beam, u, in_place);
+    if (is_meta) regather<uint32_t, BEAM>(meta + row0, out_meta + row0, parents, (int64_t)h * Tmax, beam, u, in_place);
+    else regather<u32x4, BEAM>(codes + row0 * 2, out_codes + row0 * 2, parents, (int64_t)h * Tmax * 2, beam, u, in_place);
 }
 
 // ---- attention ---------------------------------------------------------------------------------------------------------------------------

@@ -111,3 +111,22 @@ def test_finite_sums_stay_finite_with_many_slots():
     got, _ = ops.cache4_attention(torch.zeros(1, 1, 1, 64, device=DEV), c[0], c[1])
     assert T * v < 2.0 ** 119 and math.isfinite(float(got[0, 0, 0]))
     assert bool(((got / v - 1).abs() <= 40 * 2.0 ** -24).all())
+
+
+@pytest.mark.parametrize("beam", [2, 3, 4, 8])
+@pytest.mark.parametrize("t", [0, 1, 2, 30, 31, 32, 63, 64])
+def test_reorder_of_few_positions(beam, t):
+    """fewer live lanes in a wave than parents to read: the last wave of the codes (2 (t + 1) pieces) and of the meta words (t + 1)"""
+    g = torch.Generator().manual_seed(t)
+    B, T = 2, 65
+    c = rand_cache(g, 2, B * beam, 2, T)
+    rows = [b * beam + (r + 1 + b) % beam for b in range(B) for r in range(beam)]
+    before, parent = ops.Cache4(c.codes.clone(), c.meta.clone()), torch.tensor(rows, device=DEV)
+    other = rand_cache(g, 2, B * beam, 2, T)
+    was = ops.Cache4(other.codes.clone(), other.meta.clone())
+    ops.cache4_reorder(c, parent, i32(t, -1), beam, out=other)
+    ops.cache4_reorder(c, parent, i32(t, -1), beam)
+    n = t + 1
+    for got, old in ((other, was), (c, before)):
+        for a, src, o in ((got.codes, before.codes, old.codes), (got.meta, before.meta, old.meta)):
+            assert torch.equal(a[:, :, :, :n], src[:, rows, :, :n]) and torch.equal(a[:, :, :, n:], o[:, :, :, n:])
